@@ -338,6 +338,7 @@ attn_bwd_dq_kernel(const AttnBwdParams p) {
 #pragma unroll
         for (int st = 0; st < 2; ++st)
           acc[g][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ab_tr_frag<D>(kimg, dt, st, fr, fq), pb[st], acc[g][dt], 0, 0, 0);
+      if constexpr (D == 80) __builtin_amdgcn_sched_barrier(0);   // the two groups' scores alive at once spill
     }
     if (G::NBUF == 1 && t + 1 < ntiles) {
       __syncthreads();
