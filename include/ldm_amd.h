@@ -28,6 +28,8 @@ extern "C" {
 
 enum { LDM_F32 = 0, LDM_BF16 = 1 };
 
+enum { LDM_MX4 = 4, LDM_MX8 = 8 };   /* block-scaled rows: see ldm_mx_quantize */
+
 enum {
   LDM_OK = 0,
   LDM_EINVAL = -1,   /* bad argument (shape / dtype / alignment / null pointer) */
@@ -410,6 +412,52 @@ int ldm_conv1x1_nchw(const void* x, int x_dtype, const float* w, const float* bi
 /* train_latent_diffusion.py:600-601: out = uint8(255 * clamp(x / 2 + 0.5, 0, 1)), each intermediate rounded to dtype as
  * torch rounds it, the final cast truncating. */
 int ldm_image_to_uint8(const void* x, int dtype, unsigned char* out, long long n, void* stream);
+
+/* ------------------------------------------------------- block-scaled ("microscaled") rows, 4 and 8 bits */
+
+/* x (rows, cols) float32 / bfloat16, rows `ld` elements apart  ->  elements `data` and scale bytes `scale`.
+ * A row is ceil(cols / 32) blocks of 32 consecutive columns, the last one filled up with zeros; a block with largest magnitude a has
+ * one power-of-two scale 2^e, stored as the byte e + 127:
+ *   LDM_MX4  e = max(floor(log2 a) - 2, -127); elements 0, .5, 1, 1.5, 2, 3, 4, 6 and their negatives (sign bit, two exponent bits, one
+ *            mantissa bit): nearest to x / 2^e, ties to the even code, at most 6.  Two to a byte, the lower column in the lower
+ *            half: 16 bytes a block.
+ *   LDM_MX8  e = max(floor(log2 a), -127); elements q / 64, q = -127 .. 127: 64 x / 2^e to nearest even, at most 127.  32 bytes a block.
+ * A block that holds an infinity or a NaN gets the byte 255 and stands for NaN in all its 32 columns.  data: rows without gaps
+ * (16-byte aligned); scale: rows of 4 * ceil(blocks / 4) bytes, the padding bytes zero (4-byte aligned). */
+int ldm_mx_quantize(const void* x, int dtype, long long rows, int cols, long long ld, int fmt, void* data, void* scale, void* stream);
+
+/* The values that `data` / `scale` stand for -> out (rows, cols), rows `ld` elements apart; exact in float32 and (LDM_MX4, LDM_MX8: at
+ * most 7 significant bits) in bfloat16. */
+int ldm_mx_dequantize(const void* data, const void* scale, int fmt, long long rows, int cols, void* out, int dtype, long long ld,
+                      void* stream);
+
+/* The transposed values of LDM_MX4 rows in bfloat16: out[k][n], n = 0 .. rows-1, rows .. ld-1 zero (ld a multiple of 8): the filter
+ * with which ldm_conv_gemm on dY computes the input gradient of a linear layer with 4-bit weights. */
+int ldm_mx4_dequantize_t(const void* data, const void* scale, int rows, int cols, void* out, int ld, void* stream);
+
+/* GEGLU / SwiGLU whose backward pass reads an 8-bit checkpoint of the pre-activation (ldm_glu_forward / ldm_glu_backward keep it in the
+ * compute dtype; unet.py:776-790 under loss.backward()).  h (rows, 2 ff) in the paired column order of ldm_pack_weight(glu_pairs), so an
+ * LDM_MX8 block is 16 values and their 16 gates; ff a multiple of 16; contiguous, 16-byte aligned.
+ *   forward:  out (rows, ff) = value * act(gate), computed from h itself; data / scale = h in LDM_MX8
+ *   backward: dh (rows, 2 ff) from data / scale alone; out, when not NULL, receives value * act(gate) of the checkpoint again (the
+ *             operand of the next layer's weight gradient, which then need not be kept either) */
+int ldm_glu_forward_mx8(const void* h, void* out, void* data, void* scale, int dtype, long long rows, int ff, int gelu, void* stream);
+int ldm_glu_backward_mx8(const void* data, const void* scale, const void* dout, void* dh, void* out, int dtype, long long rows, int ff,
+                         int gelu, void* stream);
+
+/* out (rows, n) = x W^T + bias (bias float32, may be NULL; out float32 or bfloat16, contiguous), W (n, k) in LDM_MX4.
+ *   x_scale != NULL: x (rows, k) in LDM_MX4 as well: both operands go to the matrix cores as they are
+ *   x_scale == NULL: x (rows, k) contiguous bfloat16 (any alignment); the weights are widened to bfloat16 (exact) in registers
+ * Sums are float32.  Any rows >= 0, n >= 1, k >= 1.  x_scale == NULL reads W once for every 64 rows: meant for few rows. */
+int ldm_mx4_linear(const void* x, const void* x_scale, const void* w, const void* w_scale, const float* bias, void* out, int out_dtype,
+                   long long rows, int n, int k, void* stream);
+
+/* dw (n, k) float32 (+)= dY^T X: weight gradient of a linear layer whose input was kept in LDM_MX8.  dy (rows, n) bfloat16, contiguous,
+ * 16-byte aligned, n a multiple of 8; x8 / x8_scale (rows, k).  Sums are float32 in a fixed order (no atomics).  `workspace` of
+ * ldm_linear_wgrad_mx8_workspace_bytes (may be 0: NULL is fine then), 16-byte aligned. */
+long long ldm_linear_wgrad_mx8_workspace_bytes(long long rows, int n, int k);
+int ldm_linear_wgrad_mx8(const void* x8, const void* x8_scale, const void* dy, float* dw, long long rows, int n, int k, int accumulate,
+                         void* workspace, long long workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

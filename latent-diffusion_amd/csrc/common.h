@@ -129,6 +129,9 @@ __device__ __forceinline__ float wave_max(float v) {
 
 static inline size_t dtype_size(int dt) { return dt == LDM_BF16 ? 2 : 4; }
 static inline bool dtype_ok(int dt) { return dt == LDM_BF16 || dt == LDM_F32; }
+// Block-scaled rows (LDM_MX4 / LDM_MX8): blocks of 32 columns, scale bytes in rows of whole 32-bit words
+static inline int mx_blocks(int cols) { return (cols + 31) / 32; }
+static inline int mx_scale_stride(int cols) { return (mx_blocks(cols) + 3) / 4 * 4; }
 static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 }  // namespace ldm

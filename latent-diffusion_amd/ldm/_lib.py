@@ -16,6 +16,7 @@ import os
 import torch  # noqa: F401
 
 F32, BF16 = 0, 1
+MX4, MX8 = 4, 8
 
 EPI_BIAS, EPI_ROWVEC, EPI_RESIDUAL, EPI_SILU, EPI_GEGLU, EPI_SWIGLU, EPI_ROWSTATS, EPI_LNFOLD = 1, 2, 4, 8, 16, 32, 64, 128
 ABI_VERSION = 3
@@ -121,6 +122,14 @@ _SIGNATURES = {
     "ldm_softmax_rows": [c_void_p, C.c_longlong, C.c_longlong, c_int, c_int, c_float, c_void_p, c_int, C.c_longlong, c_void_p],
     "ldm_conv1x1_nchw": [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, C.c_longlong, c_void_p],
     "ldm_image_to_uint8": [c_void_p, c_int, c_void_p, C.c_longlong, c_void_p],
+    "ldm_mx_quantize": [c_void_p, c_int, C.c_longlong, c_int, C.c_longlong, c_int, c_void_p, c_void_p, c_void_p],
+    "ldm_mx_dequantize": [c_void_p, c_void_p, c_int, C.c_longlong, c_int, c_void_p, c_int, C.c_longlong, c_void_p],
+    "ldm_mx4_dequantize_t": [c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p],
+    "ldm_glu_forward_mx8": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, C.c_longlong, c_int, c_int, c_void_p],
+    "ldm_glu_backward_mx8": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, C.c_longlong, c_int, c_int, c_void_p],
+    "ldm_mx4_linear": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, C.c_longlong, c_int, c_int, c_void_p],
+    "ldm_linear_wgrad_mx8": [c_void_p, c_void_p, c_void_p, c_void_p, C.c_longlong, c_int, c_int, c_int, c_void_p, C.c_longlong,
+                             c_void_p],
 }
 
 # host-only size queries returning long long
@@ -129,6 +138,7 @@ _LONGLONG_QUERIES = {
     "ldm_groupnorm_backward_workspace_floats": [c_int, c_int, c_int],
     "ldm_layernorm_backward_workspace_floats": [c_int],
     "ldm_mse_workspace_floats": [C.c_longlong],
+    "ldm_linear_wgrad_mx8_workspace_bytes": [C.c_longlong, c_int, c_int],
 }
 
 EXPORTED_SYMBOLS = (["ldm_abi_version", "ldm_last_error", "ldm_conv_wgrad_workspace_bytes"] + list(_SIGNATURES)

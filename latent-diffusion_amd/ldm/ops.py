@@ -946,3 +946,265 @@ def image_to_uint8(x: torch.Tensor) -> torch.Tensor:
         _lib.check(_lib.load().ldm_image_to_uint8(x.data_ptr(), dt_code(x.dtype), out.data_ptr(), x.numel(), _stream(x)),
                    "ldm_image_to_uint8")
     return out
+
+
+# ------------------------------------------------------------------------ block-scaled ("microscaled") rows, 4 and 8 bits
+class MxTensor:
+    """Rows in blocks of 32 columns, each block under one power-of-two scale (include/ldm_amd.h ldm_mx_quantize): what
+    mx4_quantize / mx8_quantize return and what the mx operators take.
+
+    data   (*lead, 16 * blocks) uint8 for 4-bit elements, (*lead, 32 * blocks) int8 for 8-bit ones, blocks = ceil(cols / 32)
+    scale  (*lead, 4 * ceil(blocks / 4)) uint8: exponent + 127 a block (255: NaN), zero behind the last block
+    cols   columns of the rows that it stands for
+
+    Both tensors are plain storage: they may be saved, moved or concatenated along leading dimensions like any other."""
+
+    __slots__ = ("data", "scale", "cols")
+
+    def __init__(self, data: torch.Tensor, scale: torch.Tensor, cols: int):
+        blocks = (cols + 31) // 32
+        if cols < 1 or data.dim() < 1 or data.dtype not in (torch.uint8, torch.int8):
+            raise TypeError(f"MxTensor: data must be uint8 (4-bit) or int8 (8-bit) rows of at least one column (got {data.dtype})")
+        if scale.dtype != torch.uint8:
+            raise TypeError(f"MxTensor: scale must be uint8 (got {scale.dtype})")
+        width = blocks * (16 if data.dtype == torch.uint8 else 32)
+        if data.shape[-1] != width or scale.shape[-1] != (blocks + 3) // 4 * 4 or data.shape[:-1] != scale.shape[:-1]:
+            raise ValueError(f"MxTensor: {cols} columns need rows of {width} elements' bytes and {(blocks + 3) // 4 * 4} scales "
+                             f"(got {tuple(data.shape)} and {tuple(scale.shape)})")
+        if data.device != scale.device:
+            raise ValueError(f"MxTensor: data on {data.device}, scale on {scale.device}")
+        if not data.is_contiguous() or not scale.is_contiguous():
+            raise ValueError("MxTensor: data and scale must be contiguous")
+        self.data, self.scale, self.cols = data, scale, cols
+
+    @property
+    def fmt(self) -> int:
+        return _lib.MX4 if self.data.dtype == torch.uint8 else _lib.MX8
+
+    @property
+    def shape(self) -> torch.Size:
+        return torch.Size((*self.data.shape[:-1], self.cols))
+
+    @property
+    def rows(self) -> int:
+        return self.scale.numel() // self.scale.shape[-1]
+
+    def __repr__(self):
+        return f"MxTensor({'mx4' if self.fmt == _lib.MX4 else 'mx8'}, {tuple(self.shape)}, {self.data.device})"
+
+
+def _same_device(what: str, ref: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
+    for t in others:
+        if t is not None and t.device != ref.device:
+            raise ValueError(f"{what}: operands on {ref.device} and {t.device}")
+
+
+def _mx(what: str, q, fmt: int) -> None:
+    if not isinstance(q, MxTensor) or q.fmt != fmt:
+        raise TypeError(f"{what} must be an MxTensor with {'4' if fmt == _lib.MX4 else '8'}-bit elements")
+    _gpu(q.data, q.scale)
+
+
+def _mx_empty(lead, cols: int, fmt: int, device) -> MxTensor:
+    blocks = (cols + 31) // 32
+    data = torch.empty((*lead, blocks * (16 if fmt == _lib.MX4 else 32)), dtype=torch.uint8 if fmt == _lib.MX4 else torch.int8, device=device)
+    return MxTensor(data, torch.empty((*lead, (blocks + 3) // 4 * 4), dtype=torch.uint8, device=device), cols)
+
+
+def _mx_quantize(what: str, x: torch.Tensor, fmt: int) -> MxTensor:
+    _gpu(x)
+    code = dt_code(x.dtype)
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"{what}: at least one column expected, got shape {tuple(x.shape)}")
+    q = _mx_empty(x.shape[:-1], x.shape[-1], fmt, x.device)
+    if x.numel() == 0:
+        return q
+    rows, cols, ld = _rows_view(x)
+    if rows > 1 and ld < cols:
+        raise ValueError(f"{what}: rows overlap (row stride {ld} for {cols} columns)")
+    with torch.cuda.device(x.device):
+        _lib.check(_lib.load().ldm_mx_quantize(x.data_ptr(), code, rows, cols, max(ld, cols), fmt, q.data.data_ptr(), q.scale.data_ptr(),
+                                               _stream(x)), "ldm_mx_quantize")
+    return q
+
+
+def mx4_quantize(x: torch.Tensor) -> MxTensor:
+    """x (*lead, cols) float32 / bfloat16 (a dense tensor or a column slice of one) in 4-bit floats, one power-of-two scale per 32
+    columns: 4.25 bits a value.  Weights for mx4_linear, and its left operand.  A block with an infinity or a NaN becomes NaN."""
+    return _mx_quantize("mx4_quantize", x, _lib.MX4)
+
+
+def mx8_quantize(x: torch.Tensor) -> MxTensor:
+    """x (*lead, cols) float32 / bfloat16 in 8-bit whole numbers, one power-of-two scale per 32 columns: 8.25 bits a value, off by at
+    most a 64th of the block's largest magnitude.  The checkpoint that linear_wgrad_mx8 and glu_backward_mx8 read."""
+    return _mx_quantize("mx8_quantize", x, _lib.MX8)
+
+
+def mx_dequantize(q: MxTensor, dtype: torch.dtype) -> torch.Tensor:
+    """The values q stands for, float32 or bfloat16 (both hold them exactly)."""
+    if not isinstance(q, MxTensor):
+        raise TypeError("mx_dequantize: an MxTensor expected")
+    _gpu(q.data, q.scale)
+    out = torch.empty(q.shape, dtype=dtype, device=q.data.device)
+    code = dt_code(dtype)
+    if out.numel():
+        with torch.cuda.device(out.device):
+            _lib.check(_lib.load().ldm_mx_dequantize(q.data.data_ptr(), q.scale.data_ptr(), q.fmt, q.rows, q.cols, out.data_ptr(), code,
+                                                     q.cols, _stream(out)), "ldm_mx_dequantize")
+    return out
+
+
+_MX4_WIDEN_ROWS = 64        # bf16 activations: up to here the weights are widened in registers, beyond once to memory
+
+
+def _pad_cols(t: torch.Tensor, cols: int) -> torch.Tensor:
+    """(rows, c) -> (rows, cols) zero-padded copy (t itself if it has them): operands of the implicit GEMM come in whole 32 columns."""
+    if t.shape[-1] == cols:
+        return t
+    out = torch.zeros((t.shape[0], cols), dtype=t.dtype, device=t.device)
+    out[:, :t.shape[-1]] = t
+    return out
+
+
+def mx4_linear(x, w: MxTensor, bias: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """x W^T + bias for 4-bit weights w (n, k): (*lead, n), float32 sums.  x: an MxTensor with 4-bit elements (*lead, k) -- both
+    operands go to the matrix cores as they are -- or bfloat16 (*lead, k), contiguous, multiplied as it is with the weights widened
+    (exactly) to bfloat16.  bias: float32 (n,).  out_dtype: bfloat16 (default) or float32."""
+    _mx("mx4_linear: w", w, _lib.MX4)
+    if w.data.dim() != 2:
+        raise ValueError(f"mx4_linear: w must be (n, k), got {tuple(w.shape)}")
+    n, k = w.shape
+    mx = isinstance(x, MxTensor)
+    if mx:
+        _mx("mx4_linear: x", x, _lib.MX4)
+    else:
+        _gpu(x)
+        if x.dtype != torch.bfloat16:
+            raise TypeError(f"mx4_linear: x must be bfloat16 or an MxTensor (got {x.dtype})")
+        if not x.is_contiguous():
+            raise ValueError("mx4_linear: x must be contiguous")
+    if len(x.shape) < 1 or x.shape[-1] != k:
+        raise ValueError(f"mx4_linear: x {tuple(x.shape)} does not match w {tuple(w.shape)}")
+    odt = out_dtype or torch.bfloat16
+    code = dt_code(odt)
+    _gpu(bias)
+    _f32_dense("mx4_linear: bias", bias, n)
+    xt = x.data if mx else x
+    _same_device("mx4_linear", xt, w.data, bias)
+    lead = x.shape[:-1]
+    rows = xt.numel() // xt.shape[-1]
+    if not mx and rows > _MX4_WIDEN_ROWS:
+        # many rows: the weights are read by many workgroups, so widening them once costs less than in every one of them
+        kp = (k + 31) // 32 * 32
+        wide = torch.empty((n, kp), dtype=torch.bfloat16, device=x.device)
+        with torch.cuda.device(x.device):
+            _lib.check(_lib.load().ldm_mx_dequantize(w.data.data_ptr(), w.scale.data_ptr(), _lib.MX4, n, kp, wide.data_ptr(), BF16, kp,
+                                                     _stream(x)), "ldm_mx_dequantize")
+        return conv_gemm(_pad_cols(x.reshape(rows, k), kp), wide, bias=bias, out_dtype=odt).view(*lead, n)
+    out = torch.empty((*lead, n), dtype=odt, device=xt.device)
+    if rows:
+        with torch.cuda.device(xt.device):
+            _lib.check(_lib.load().ldm_mx4_linear(xt.data_ptr(), x.scale.data_ptr() if mx else 0, w.data.data_ptr(), w.scale.data_ptr(),
+                                                  _ptr(bias), out.data_ptr(), code, rows, n, k, _stream(xt)), "ldm_mx4_linear")
+    return out
+
+
+def mx4_linear_dgrad(dy: torch.Tensor, w: MxTensor) -> torch.Tensor:
+    """Input gradient of mx4_linear(x, w): dy W, (*lead, n) -> (*lead, k), bfloat16, float32 sums.  The weights themselves have no
+    gradient: they are frozen (what is trained around them -- biases, norms, added low-rank layers -- has its own operators)."""
+    _mx("mx4_linear_dgrad: w", w, _lib.MX4)
+    if w.data.dim() != 2:
+        raise ValueError(f"mx4_linear_dgrad: w must be (n, k), got {tuple(w.shape)}")
+    _gpu(dy)
+    n, k = w.shape
+    if dy.dtype != torch.bfloat16:
+        raise TypeError(f"mx4_linear_dgrad: dy must be bfloat16 (got {dy.dtype})")
+    if dy.dim() < 1 or dy.shape[-1] != n or not dy.is_contiguous():
+        raise ValueError(f"mx4_linear_dgrad: dy must be a contiguous (..., {n}) tensor, got {tuple(dy.shape)}")
+    _same_device("mx4_linear_dgrad", dy, w.data)
+    rows = dy.numel() // n
+    if rows == 0:
+        return torch.empty((*dy.shape[:-1], k), dtype=dy.dtype, device=dy.device)
+    np_ = (n + 31) // 32 * 32
+    wt = torch.empty((k, np_), dtype=torch.bfloat16, device=dy.device)
+    with torch.cuda.device(dy.device):
+        _lib.check(_lib.load().ldm_mx4_dequantize_t(w.data.data_ptr(), w.scale.data_ptr(), n, k, wt.data_ptr(), np_, _stream(dy)),
+                   "ldm_mx4_dequantize_t")
+    return conv_gemm(_pad_cols(dy.reshape(rows, n), np_), wt).view(*dy.shape[:-1], k)
+
+
+def _glu_kind(what: str, act: str) -> int:
+    if act not in ("geglu", "swiglu"):
+        raise ValueError(f"{what}: Unsupported activation function: {act}")
+    return 1 if act == "geglu" else 0
+
+
+def glu_forward_mx8(h: torch.Tensor, act: str):
+    """glu_forward that leaves an 8-bit checkpoint of h for the backward pass: (out (.., ff), h in mx8), one pass over h.
+    h (.., 2 ff) in the packed (paired) column order, ff a multiple of 16; out is computed from h itself."""
+    gelu = _glu_kind("glu_forward_mx8", act)
+    _gpu(h)
+    code = dt_code(h.dtype)
+    _same_dtype_dense("glu_forward_mx8", h)
+    if h.dim() < 1 or h.shape[-1] < 32 or h.shape[-1] % 32:
+        raise ValueError(f"glu_forward_mx8: h needs a multiple of 32 columns, got {tuple(h.shape)}")
+    ff = h.shape[-1] // 2
+    out = torch.empty((*h.shape[:-1], ff), dtype=h.dtype, device=h.device)
+    q = _mx_empty(h.shape[:-1], 2 * ff, _lib.MX8, h.device)
+    with torch.cuda.device(h.device):
+        _lib.check(_lib.load().ldm_glu_forward_mx8(h.data_ptr(), out.data_ptr(), q.data.data_ptr(), q.scale.data_ptr(), code,
+                                                   h.numel() // (2 * ff), ff, gelu, _stream(h)), "ldm_glu_forward_mx8")
+    return out, q
+
+
+def glu_backward_mx8(h8: MxTensor, dout: torch.Tensor, act: str, recompute: bool = False):
+    """Gradient of the gated activation from its checkpoint alone: dh (.., 2 ff) in dout's dtype.  recompute=True: (dh, out) with out
+    the activation of the checkpoint, the next layer's input for its weight gradient."""
+    gelu = _glu_kind("glu_backward_mx8", act)
+    _mx("glu_backward_mx8: h8", h8, _lib.MX8)
+    _gpu(dout)
+    code = dt_code(dout.dtype)
+    _same_dtype_dense("glu_backward_mx8", dout)
+    if h8.cols % 32 or tuple(dout.shape) != (*h8.shape[:-1], h8.cols // 2):
+        raise ValueError(f"glu_backward_mx8: dout {tuple(dout.shape)} does not match the checkpoint {tuple(h8.shape)}")
+    _same_device("glu_backward_mx8", dout, h8.data)
+    ff = h8.cols // 2
+    dh = torch.empty(tuple(h8.shape), dtype=dout.dtype, device=dout.device)
+    out = torch.empty(tuple(dout.shape), dtype=dout.dtype, device=dout.device) if recompute else None
+    with torch.cuda.device(dout.device):
+        _lib.check(_lib.load().ldm_glu_backward_mx8(h8.data.data_ptr(), h8.scale.data_ptr(), dout.data_ptr(), dh.data_ptr(), _ptr(out), code,
+                                                    h8.rows, ff, gelu, _stream(dout)), "ldm_glu_backward_mx8")
+    return (dh, out) if recompute else dh
+
+
+def linear_wgrad_mx8(x8: MxTensor, dy: torch.Tensor, *, out: Optional[torch.Tensor] = None, accumulate: Optional[bool] = None) -> torch.Tensor:
+    """Weight gradient dY^T X (n, k) float32 of a linear layer whose input was kept as an 8-bit checkpoint x8 (*lead, k); dy (*lead, n)
+    bfloat16.  ``out`` / ``accumulate`` as conv_wgrad: an existing gradient to accumulate into, or a buffer to overwrite."""
+    _mx("linear_wgrad_mx8: x8", x8, _lib.MX8)
+    _gpu(dy, out)
+    if dy.dtype != torch.bfloat16:
+        raise TypeError(f"linear_wgrad_mx8: dy must be bfloat16 (got {dy.dtype})")
+    if dy.dim() < 1 or dy.shape[-1] < 1 or dy.shape[:-1] != x8.shape[:-1] or not dy.is_contiguous():
+        raise ValueError(f"linear_wgrad_mx8: dy must be a contiguous {(*x8.shape[:-1], 'n')} tensor, got {tuple(dy.shape)}")
+    _same_device("linear_wgrad_mx8", dy, x8.data, out)
+    n, k, rows = dy.shape[-1], x8.cols, x8.rows
+    if accumulate is None:
+        accumulate = out is not None
+    if out is None:
+        accumulate = False
+        out = torch.empty((n, k), dtype=torch.float32, device=dy.device)
+    elif out.dtype != torch.float32 or tuple(out.shape) != (n, k) or not out.is_contiguous():
+        raise ValueError(f"linear_wgrad_mx8: out must be a contiguous float32 tensor of shape {(n, k)}")
+    if rows == 0:
+        return out if accumulate else out.zero_()
+    npad = (n + 7) // 8 * 8
+    if npad != n:               # the kernel fetches dy in 16-byte pieces: odd widths go through a padded copy
+        full = linear_wgrad_mx8(x8, _pad_cols(dy.reshape(rows, n), npad).view(*dy.shape[:-1], npad))[:n]
+        return out.add_(full) if accumulate else out.copy_(full)
+    lib = _lib.load()
+    with torch.cuda.device(dy.device):
+        need = lib.ldm_linear_wgrad_mx8_workspace_bytes(rows, n, k)
+        ws = _wgrad_workspace(dy.device, need) if need else None
+        _lib.check(lib.ldm_linear_wgrad_mx8(x8.data.data_ptr(), x8.scale.data_ptr(), dy.data_ptr(), out.data_ptr(), rows, n, k,
+                                            1 if accumulate else 0, _ptr(ws), need, _stream(dy)), "ldm_linear_wgrad_mx8")
+    return out

@@ -150,7 +150,8 @@ def build(force=False, verbose=False):
     stamp = _stamp()
     if not force and os.path.exists(OUT) and os.path.exists(stamp_file) and open(stamp_file).read() == stamp:
         return OUT
-    flags = ["-std=c++20", "-O2", "-g1", "-fPIC", "-w", "-fno-strict-aliasing", "-march=native", "-ffp-contract=fast",
+    # -mno-avx512bf16: the host's float32 -> bfloat16 instruction flushes subnormals, v_cvt_pk_bf16_f32 does not
+    flags = ["-std=c++20", "-O2", "-g1", "-fPIC", "-w", "-fno-strict-aliasing", "-march=native", "-mno-avx512bf16", "-ffp-contract=fast",
              "-I", os.path.join(HERE, "shim"), "-I", HERE, "-I", CSRC]
     objs, procs = [], []
     for src in _sources():

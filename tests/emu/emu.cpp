@@ -193,6 +193,37 @@ void run_op(Op op, Fiber** lanes, int n) {
       }
       break;
     }
+    // A, B: lane l holds row / column l % R and the 32 consecutive k from 32 (l / R), under one scale byte; C/D as for the
+    // unscaled instruction of that shape
+    case OP_MFMA_SCALE_32x32x64:
+    case OP_MFMA_SCALE_16x16x128: {
+      need_full(n, "v_mfma_scale_f32 with a partial EXEC mask");
+      const int R = op == OP_MFMA_SCALE_32x32x64 ? 32 : 16, K = 32 * (64 / R);
+      static double A[32][128], Bt[32][128];
+      auto val = [](unsigned char n4, unsigned char code) {
+        static const double grid[8] = {0, 0.5, 1, 1.5, 2, 3, 4, 6};
+        const double v = code == 255 ? (double)NAN : ldexp(grid[n4 & 7], (int)code - 127);
+        return (n4 & 8) ? -v : v;
+      };
+      for (int l = 0; l < 64; ++l) {
+        const ScaleMfmaIn* in = static_cast<const ScaleMfmaIn*>(lanes[l]->in);
+        for (int j = 0; j < 32; ++j) {
+          A[l % R][32 * (l / R) + j] = val(in->a[j / 2] >> (4 * (j & 1)) & 15, in->sa);
+          Bt[l % R][32 * (l / R) + j] = val(in->b[j / 2] >> (4 * (j & 1)) & 15, in->sb);
+        }
+      }
+      for (int l = 0; l < 64; ++l) {
+        const ScaleMfmaIn* in = static_cast<const ScaleMfmaIn*>(lanes[l]->in);
+        float* out = static_cast<float*>(lanes[l]->out);
+        for (int r = 0; r < R * R / 64; ++r) {
+          const int row = R == 32 ? 8 * (r / 4) + 4 * (l / 32) + r % 4 : 4 * (l / 16) + r;
+          double s = 0;
+          for (int k = 0; k < K; ++k) s += A[row][k] * Bt[l % R][k];
+          out[r] = in->c[r] + (float)s;
+        }
+      }
+      break;
+    }
     case OP_SHFL: {
       const Fiber* by_lane[64] = {};
       for (int i = 0; i < n; ++i) by_lane[lanes[i]->info.lane] = lanes[i];

@@ -43,9 +43,14 @@ enum Op : int {
   OP_PERMLANE32_SWAP,
   OP_DS_READ_TR16_B64,
   OP_WAVE_BARRIER,
+  OP_MFMA_SCALE_32x32x64,
+  OP_MFMA_SCALE_16x16x128,
 };
 
 struct ShflIn { uint64_t value; int src; int width; int mode; };   // mode 0: index, 1: xor, 2: down, 3: up
+
+// one lane's operands of a block-scaled MFMA on 4-bit floats: 32 elements of each operand, their scale bytes, the accumulator
+struct ScaleMfmaIn { unsigned char a[16], b[16], sa, sb; float c[16]; };
 
 void wave_op(Op op, const void* tag, const void* in, void* out);     // blocks the calling lane until the wave runs the op
 void barrier();                                                       // s_barrier: no memory wait of its own

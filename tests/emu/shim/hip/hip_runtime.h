@@ -202,8 +202,70 @@ static inline unsigned raw_buffer_load_b32(rsrc_t rs, int voff, int soff, int) {
   return r;
 }
 
+// quad permutations of v_mov_b32_dpp (the only DPP controls the kernels use)
+static inline __attribute__((always_inline)) int update_dpp(int /*old*/, int src, int ctrl, int, int, bool) {
+  if (ctrl > 0xFF) abort();
+  const int l = me().lane;
+  return shfl_any(src, (l & ~3) | ((ctrl >> (2 * (l & 3))) & 3), 64, 0);
+}
+
+// 4-bit floats (1 sign, 2 exponent, 1 mantissa bit) under a power-of-two scale: the scale operand's exponent field is taken as it
+// is (0: 2^-127, 255: NaN); rounding to nearest even, held to 6
+static inline double e8m0(float s) {
+  const int code = (int)((__float_as_uint(s) >> 23) & 255);
+  return code == 255 ? (double)NAN : ldexp(1.0, code - 127);
+}
+static inline unsigned fp4_of(double y) {
+  const double a = fabs(y);
+  const unsigned c = (a > 0.25) + (a >= 0.75) + (a > 1.25) + (a >= 1.75) + (a > 2.5) + (a >= 3.5) + (a > 5.0);
+  return c | (std::signbit(y) ? 8u : 0u);
+}
+static inline float fp4_to(unsigned n) {
+  static const float grid[8] = {0.f, 0.5f, 1.f, 1.5f, 2.f, 3.f, 4.f, 6.f};
+  return (n & 8) ? -grid[n & 7] : grid[n & 7];
+}
+static inline unsigned cvt_pk_fp4_f32(unsigned old, float a, float b, float s, int sel) {
+  const double u = e8m0(s);
+  const unsigned byte = fp4_of(a / u) | fp4_of(b / u) << 4;
+  return (old & ~(0xFFu << (8 * sel))) | byte << (8 * sel);
+}
+typedef float f32x2_emu __attribute__((ext_vector_type(2)));
+static inline f32x2_emu cvt_pk_f32_fp4(unsigned w, float s, int sel) {
+  const unsigned byte = w >> (8 * sel);
+  const double u = e8m0(s);
+  return f32x2_emu{(float)(fp4_to(byte & 15) * u), (float)(fp4_to((byte >> 4) & 15) * u)};
+}
+typedef __bf16 bf16x2_emu __attribute__((ext_vector_type(2)));
+static inline bf16x2_emu cvt_pk_bf16_fp4(unsigned w, float s, int sel) {
+  const f32x2_emu v = cvt_pk_f32_fp4(w, s, sel);
+  return bf16x2_emu{__truncsfbf2(v[0]), __truncsfbf2(v[1])};
+}
+
+// v_mfma_scale_f32_{32x32x64,16x16x128}_f8f6f4 on 4-bit floats (format code 4): the first four registers of an operand are read,
+// `sel` picks the scale byte
+template <int OP, int ROWS, typename A, typename C>
+EMU_NOINLINE C mfma_scale_fp4(A a, A b, C c, int fa, int fb, int sel_a, int sa, int sel_b, int sb) {
+  static_assert(sizeof(A) == 32 && sizeof(C) == ROWS * ROWS / 16, "operand sizes");
+  if (fa != 4 || fb != 4) abort();
+  ScaleMfmaIn in;
+  memcpy(in.a, &a, 16);
+  memcpy(in.b, &b, 16);
+  memcpy(in.c, &c, sizeof(C));
+  in.sa = (unsigned char)((unsigned)sa >> (8 * sel_a));
+  in.sb = (unsigned char)((unsigned)sb >> (8 * sel_b));
+  C out;
+  wave_op((Op)OP, __builtin_return_address(0), &in, &out);
+  return out;
+}
+
 }  // namespace emu
 
+#define __builtin_amdgcn_update_dpp ::emu::update_dpp
+#define __builtin_amdgcn_cvt_scalef32_pk_fp4_f32 ::emu::cvt_pk_fp4_f32
+#define __builtin_amdgcn_cvt_scalef32_pk_f32_fp4 ::emu::cvt_pk_f32_fp4
+#define __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4 ::emu::cvt_pk_bf16_fp4
+#define __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4 (::emu::mfma_scale_fp4<::emu::OP_MFMA_SCALE_32x32x64, 32>)
+#define __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4 (::emu::mfma_scale_fp4<::emu::OP_MFMA_SCALE_16x16x128, 16>)
 #define __amdgpu_buffer_rsrc_t ::emu::rsrc_t
 #define __builtin_amdgcn_make_buffer_rsrc ::emu::make_buffer_rsrc
 #define __builtin_amdgcn_raw_ptr_buffer_load_lds ::emu::raw_ptr_buffer_load_lds
