@@ -32,7 +32,8 @@ def _gpu(*ts):
 
 
 def _stream(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+    # the raw handle: 0.1 us a call against 2 us for building torch.cuda.current_stream(t.device) around it
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
 def _ptr(t: Optional[torch.Tensor]) -> int:
@@ -1007,8 +1008,25 @@ def _mx(what: str, q, fmt: int) -> None:
 
 def _mx_empty(lead, cols: int, fmt: int, device) -> MxTensor:
     blocks = (cols + 31) // 32
-    data = torch.empty((*lead, blocks * (16 if fmt == _lib.MX4 else 32)), dtype=torch.uint8 if fmt == _lib.MX4 else torch.int8, device=device)
-    return MxTensor(data, torch.empty((*lead, (blocks + 3) // 4 * 4), dtype=torch.uint8, device=device), cols)
+    q = MxTensor.__new__(MxTensor)          # laid out here: nothing for the constructor to check
+    q.data = torch.empty((*lead, blocks * (16 if fmt == _lib.MX4 else 32)), dtype=torch.uint8 if fmt == _lib.MX4 else torch.int8,
+                         device=device)
+    q.scale = torch.empty((*lead, (blocks + 3) // 4 * 4), dtype=torch.uint8, device=device)
+    q.cols = cols
+    return q
+
+
+def _call(t: torch.Tensor, entry: str, *args) -> None:
+    """The C entry on t's device and its current stream.  These calls take a few microseconds on the GPU for few rows, so the device
+    is switched only where it is not the current one (1.3 us)."""
+    fn = getattr(_lib.load(), entry)
+    if 0 <= t.get_device() == torch.cuda.current_device():
+        rc = fn(*args, _stream(t))
+    else:
+        with torch.cuda.device(t.device):
+            rc = fn(*args, _stream(t))
+    if rc:
+        _lib.check(rc, entry)
 
 
 def _mx_quantize(what: str, x: torch.Tensor, fmt: int) -> MxTensor:
@@ -1022,9 +1040,7 @@ def _mx_quantize(what: str, x: torch.Tensor, fmt: int) -> MxTensor:
     rows, cols, ld = _rows_view(x)
     if rows > 1 and ld < cols:
         raise ValueError(f"{what}: rows overlap (row stride {ld} for {cols} columns)")
-    with torch.cuda.device(x.device):
-        _lib.check(_lib.load().ldm_mx_quantize(x.data_ptr(), code, rows, cols, max(ld, cols), fmt, q.data.data_ptr(), q.scale.data_ptr(),
-                                               _stream(x)), "ldm_mx_quantize")
+    _call(x, "ldm_mx_quantize", x.data_ptr(), code, rows, cols, max(ld, cols), fmt, q.data.data_ptr(), q.scale.data_ptr())
     return q
 
 
@@ -1048,9 +1064,7 @@ def mx_dequantize(q: MxTensor, dtype: torch.dtype) -> torch.Tensor:
     out = torch.empty(q.shape, dtype=dtype, device=q.data.device)
     code = dt_code(dtype)
     if out.numel():
-        with torch.cuda.device(out.device):
-            _lib.check(_lib.load().ldm_mx_dequantize(q.data.data_ptr(), q.scale.data_ptr(), q.fmt, q.rows, q.cols, out.data_ptr(), code,
-                                                     q.cols, _stream(out)), "ldm_mx_dequantize")
+        _call(out, "ldm_mx_dequantize", q.data.data_ptr(), q.scale.data_ptr(), q.fmt, q.rows, q.cols, out.data_ptr(), code, q.cols)
     return out
 
 
@@ -1097,15 +1111,12 @@ def mx4_linear(x, w: MxTensor, bias: Optional[torch.Tensor] = None, out_dtype: O
         # many rows: the weights are read by many workgroups, so widening them once costs less than in every one of them
         kp = (k + 31) // 32 * 32
         wide = torch.empty((n, kp), dtype=torch.bfloat16, device=x.device)
-        with torch.cuda.device(x.device):
-            _lib.check(_lib.load().ldm_mx_dequantize(w.data.data_ptr(), w.scale.data_ptr(), _lib.MX4, n, kp, wide.data_ptr(), BF16, kp,
-                                                     _stream(x)), "ldm_mx_dequantize")
+        _call(x, "ldm_mx_dequantize", w.data.data_ptr(), w.scale.data_ptr(), _lib.MX4, n, kp, wide.data_ptr(), BF16, kp)
         return conv_gemm(_pad_cols(x.reshape(rows, k), kp), wide, bias=bias, out_dtype=odt).view(*lead, n)
     out = torch.empty((*lead, n), dtype=odt, device=xt.device)
     if rows:
-        with torch.cuda.device(xt.device):
-            _lib.check(_lib.load().ldm_mx4_linear(xt.data_ptr(), x.scale.data_ptr() if mx else 0, w.data.data_ptr(), w.scale.data_ptr(),
-                                                  _ptr(bias), out.data_ptr(), code, rows, n, k, _stream(xt)), "ldm_mx4_linear")
+        _call(xt, "ldm_mx4_linear", xt.data_ptr(), x.scale.data_ptr() if mx else 0, w.data.data_ptr(), w.scale.data_ptr(), _ptr(bias),
+              out.data_ptr(), code, rows, n, k)
     return out
 
 
@@ -1127,9 +1138,7 @@ def mx4_linear_dgrad(dy: torch.Tensor, w: MxTensor) -> torch.Tensor:
         return torch.empty((*dy.shape[:-1], k), dtype=dy.dtype, device=dy.device)
     np_ = (n + 31) // 32 * 32
     wt = torch.empty((k, np_), dtype=torch.bfloat16, device=dy.device)
-    with torch.cuda.device(dy.device):
-        _lib.check(_lib.load().ldm_mx4_dequantize_t(w.data.data_ptr(), w.scale.data_ptr(), n, k, wt.data_ptr(), np_, _stream(dy)),
-                   "ldm_mx4_dequantize_t")
+    _call(dy, "ldm_mx4_dequantize_t", w.data.data_ptr(), w.scale.data_ptr(), n, k, wt.data_ptr(), np_)
     return conv_gemm(_pad_cols(dy.reshape(rows, n), np_), wt).view(*dy.shape[:-1], k)
 
 
@@ -1151,9 +1160,8 @@ def glu_forward_mx8(h: torch.Tensor, act: str):
     ff = h.shape[-1] // 2
     out = torch.empty((*h.shape[:-1], ff), dtype=h.dtype, device=h.device)
     q = _mx_empty(h.shape[:-1], 2 * ff, _lib.MX8, h.device)
-    with torch.cuda.device(h.device):
-        _lib.check(_lib.load().ldm_glu_forward_mx8(h.data_ptr(), out.data_ptr(), q.data.data_ptr(), q.scale.data_ptr(), code,
-                                                   h.numel() // (2 * ff), ff, gelu, _stream(h)), "ldm_glu_forward_mx8")
+    _call(h, "ldm_glu_forward_mx8", h.data_ptr(), out.data_ptr(), q.data.data_ptr(), q.scale.data_ptr(), code, h.numel() // (2 * ff), ff,
+          gelu)
     return out, q
 
 
@@ -1171,9 +1179,8 @@ def glu_backward_mx8(h8: MxTensor, dout: torch.Tensor, act: str, recompute: bool
     ff = h8.cols // 2
     dh = torch.empty(tuple(h8.shape), dtype=dout.dtype, device=dout.device)
     out = torch.empty(tuple(dout.shape), dtype=dout.dtype, device=dout.device) if recompute else None
-    with torch.cuda.device(dout.device):
-        _lib.check(_lib.load().ldm_glu_backward_mx8(h8.data.data_ptr(), h8.scale.data_ptr(), dout.data_ptr(), dh.data_ptr(), _ptr(out), code,
-                                                    h8.rows, ff, gelu, _stream(dout)), "ldm_glu_backward_mx8")
+    _call(dout, "ldm_glu_backward_mx8", h8.data.data_ptr(), h8.scale.data_ptr(), dout.data_ptr(), dh.data_ptr(), _ptr(out), code, h8.rows,
+          ff, gelu)
     return (dh, out) if recompute else dh
 
 
@@ -1201,10 +1208,9 @@ def linear_wgrad_mx8(x8: MxTensor, dy: torch.Tensor, *, out: Optional[torch.Tens
     if npad != n:               # the kernel fetches dy in 16-byte pieces: odd widths go through a padded copy
         full = linear_wgrad_mx8(x8, _pad_cols(dy.reshape(rows, n), npad).view(*dy.shape[:-1], npad))[:n]
         return out.add_(full) if accumulate else out.copy_(full)
-    lib = _lib.load()
-    with torch.cuda.device(dy.device):
-        need = lib.ldm_linear_wgrad_mx8_workspace_bytes(rows, n, k)
-        ws = _wgrad_workspace(dy.device, need) if need else None
-        _lib.check(lib.ldm_linear_wgrad_mx8(x8.data.data_ptr(), x8.scale.data_ptr(), dy.data_ptr(), out.data_ptr(), rows, n, k,
-                                            1 if accumulate else 0, _ptr(ws), need, _stream(dy)), "ldm_linear_wgrad_mx8")
+    need = _lib.load().ldm_linear_wgrad_mx8_workspace_bytes(rows, n, k)
+    # from the allocator, not kept: a graph that captured the call owns its own, and no other call or graph writes to it
+    ws = torch.empty(need, dtype=torch.uint8, device=dy.device) if need else None
+    _call(dy, "ldm_linear_wgrad_mx8", x8.data.data_ptr(), x8.scale.data_ptr(), dy.data_ptr(), out.data_ptr(), rows, n, k,
+          1 if accumulate else 0, _ptr(ws), need)
     return out
