@@ -7,10 +7,10 @@
 // of what the bf16 activation would.
 //
 // The contraction runs over the rows of both operands.  A workgroup of 8 waves owns T0 columns of dY x T1 columns of x and walks its
-// share of the rows 32 a step: dY goes to LDS by LDS-DMA (two steps ahead), x through registers -- loaded two steps ahead, widened
-// and written one step ahead, once per workgroup, under the MFMAs -- and both operands' fragments are read transposed
-// (ds_read_b64_tr_b16, the same permutation of the rows on both sides).  One barrier a step, three slots.  The rows are split over
-// blockIdx.y where there are few tiles; the partial tiles are added by a second kernel in a fixed order (no atomics).
+// share of the rows 64 a step, double-buffered: dY goes to LDS by LDS-DMA one step ahead; x goes there by LDS-DMA two steps ahead as it
+// is stored, and the thread that fetched 16 of its elements widens them into the bf16 image one step ahead.  Both operands' fragments
+// are read transposed (ds_read_b64_tr_b16, the same permutation of the rows on both sides).  The rows are split over blockIdx.y where
+// there are few tiles; the partial tiles are added by a second kernel in a fixed order (no atomics).
 #include "common.h"
 
 #include <type_traits>
@@ -32,19 +32,55 @@ struct WgradMx8Params {
   int tiles_n, tiles_k;
   int steps_per_split, splits;
   int accumulate;              // direct form only
+  int vec_out;                 // 16-byte stores of `out` are legal
 };
 
-constexpr int WM8_MS = 32;     // rows a step: one MFMA contraction block
+constexpr int WM8_MS = 64;     // rows a step: two MFMA contraction blocks
 
 // 16-byte chunks of an image row are swizzled in pairs by row so that the eight rows a transposed read touches lie in eight different
-// 32-byte columns of the LDS line: rows of 512 bytes all start at bank 0 (flip by row & 7), rows of 640 bytes alternate between
-// the line's halves (flip by (row >> 1) & 3, inside aligned groups of eight chunks)
+// 32-byte columns of the 256-byte LDS line.  Rows of a multiple of 256 bytes all start at its first column (flip the pair by row & 7);
+// rows of 128 bytes more alternate between its halves (by (row >> 1) & 3, inside aligned groups of four pairs); rows of 64 bytes more
+// start at every second column in turn (by (row >> 2) & 1, inside groups of two).
 template <int T>
-__device__ __forceinline__ int wm8_swz(int row) { return T == 256 ? (row & 7) << 1 : ((row >> 1) & 3) << 1; }
+__device__ __forceinline__ int wm8_swz(int row) {
+  return T % 128 == 0 ? (row & 7) << 1 : T % 64 == 0 ? ((row >> 1) & 3) << 1 : ((row >> 2) & 1) << 1;
+}
+// pairs in a group that the swizzle stays inside of: fragment i of a row is fragment i % that many, and whole groups further on
+template <int T, int F>
+constexpr int wm8_distinct() { return T % 128 == 0 ? F : T % 64 == 0 ? 4 : 2; }
 
 __device__ __forceinline__ void wm8_dma16(const void* base, int bytes, unsigned char* lds, unsigned voff) {
   const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, 0x00020000);
   __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)lds, 16, voff, 0, 0, 0);
+}
+
+__device__ __forceinline__ void wm8_dma4(const void* base, int bytes, unsigned char* lds, unsigned voff) {
+  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, 0x00020000);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)lds, 4, voff, 0, 0, 0);
+}
+// transposed LDS read; the caller waits before it uses the value
+template <int OFF>
+__device__ __forceinline__ void tr_read(bf16x4_t& v, unsigned addr) {
+  asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2" : "=v"(v) : "v"(addr), "n"(OFF) : "memory");
+}
+
+// min(4, left) values to (or added to) dst.  The adding form is kept out of line: 25 copies of it would be fetched once each from far memory.
+__device__ __attribute__((noinline)) void wm8_add(float* dst, int left, f32x4_t v) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (e < left) dst[e] += v[e];
+}
+__device__ __forceinline__ void wm8_store(float* dst, int left, f32x4_t v, int vec, int accumulate) {
+  if (left <= 0) return;
+  if (accumulate) {
+    wm8_add(dst, left, v);
+  } else if (vec) {                                        // k and the base are multiples of four floats: all four or none
+    *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < left) dst[e] = v[e];
+  }
 }
 
 template <int T0, int T1, int W0, int W1>
@@ -53,98 +89,132 @@ linear_wgrad_mx8_kernel(const WgradMx8Params p) {
   constexpr unsigned OOB = 0x80000000u;
   constexpr int F0 = T0 / W0 / 16, F1 = T1 / W1 / 16;
   constexpr int IMG0 = WM8_MS * T0 * 2, IMG1 = WM8_MS * T1 * 2, SLOT = IMG0 + IMG1;
-  constexpr int NI0 = IMG0 / 1024;                         // DMA instructions of the workgroup a step
-  constexpr int JMAX = (NI0 + 7) / 8, JMIN = NI0 / 8;
+  constexpr int ND = IMG0 / 1024 / 8;                      // dY DMA instructions of a wave a step
   constexpr int UPR = T1 / 16;                             // units of 16 columns (half a block) a row of x
-  constexpr int UMAX = (WM8_MS * UPR + 511) / 512;         // units a thread stages a step
-  constexpr int UFULL = WM8_MS * UPR / 512;
-  static_assert(W0 * W1 == 8 && (WM8_MS * UPR) % 64 == 0, "tile / waves mismatch");
+  constexpr int UNITS = WM8_MS * UPR, UMAX = (UNITS + 511) / 512, UFULL = UNITS / 512;
+  constexpr int RAW = UNITS * 20;
+  static_assert(W0 * W1 == 8 && IMG0 % 8192 == 0 && UNITS % 64 == 0 && UMAX <= 2, "tile / waves mismatch");
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int w0 = wave / W1, w1 = wave % W1;
-  const int tn = blockIdx.x % p.tiles_n, tk = blockIdx.x / p.tiles_n;
+  // Workgroups b and b + 8 share an XCD.  Every XCD gets a contiguous run of (split, tile): the tiles of one range of rows then share its
+  // rows of dY and x in one L2 (spread over the XCDs, x came over the fabric once for each of them: 265 MB for 180 MB of operands)
+  const int blocks = gridDim.x, q8 = blocks >> 3, r8 = blocks & 7, xcd = blockIdx.x & 7;
+  const int work = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + ((int)blockIdx.x >> 3);
+  const int tiles = p.tiles_n * p.tiles_k, split = work / tiles, tile = work - split * tiles;
+  const int tn = tile % p.tiles_n, tk = tile / p.tiles_n;
   const int n0 = tn * T0, k0 = tk * T1;
   const int total_steps = (int)((p.rows + WM8_MS - 1) / WM8_MS);
-  const int step_begin = blockIdx.y * p.steps_per_split;
+  const int step_begin = split * p.steps_per_split;
   const int nsteps = min(step_begin + p.steps_per_split, total_steps) - step_begin;
 
-  // dY: the descriptor moves 32 rows a step and ends with the matrix (rows past it read as zeros); lane offsets are constant
-  unsigned dvoff[JMAX];
+  // ---- loads.  dY: the descriptor moves 64 rows a step and ends with the matrix (rows past it read as zeros); lane offsets are constant.
+  // x: units of 16 elements of one row, and the 32-bit word with their block's scale byte, into a place of the thread's own (two steps'
+  // worth); rows past the end and blocks past the row read as zeros.
+  unsigned dvoff[ND];
 #pragma unroll
-  for (int j = 0; j < JMAX; ++j) {
+  for (int j = 0; j < ND; ++j) {
     const int c = (j * 8 + wave) * 64 + lane, row = c / (T0 / 8), phys = c - row * (T0 / 8);
     const int col = n0 + (phys ^ wm8_swz<T0>(row)) * 8;
     dvoff[j] = col < p.n ? ((unsigned)row * p.n + col) * 2u : OOB;
   }
-  const long long dy_step = (long long)WM8_MS * p.n * 2;
-  const char* dy_ptr = p.dy + (long long)step_begin * dy_step;
-  long long dy_left = (p.rows - (long long)step_begin * WM8_MS) * p.n * 2;
-  auto stage_dy = [&](int slot) {
-    const int bytes = dy_left > 0x7fffffffLL ? 0x7fffffff : (int)dy_left;
+  const int dy_row = p.n * 2, xd_row = p.blocks * 32;
+  auto rows_of = [&](int step) {                           // rows of a step inside the matrix
+    return step == total_steps - 1 ? (int)(p.rows - (long long)step * WM8_MS) : WM8_MS;
+  };
+  // the loads of the step being issued: set up once a step, then issued one instruction at a time between MFMAs
+  const char* dy_ptr = p.dy + (long long)step_begin * WM8_MS * dy_row;
+  int dy_step = step_begin, dy_bytes = 0;
+  unsigned char* dy_dst = nullptr;
+  auto begin_dy = [&](int slot) {
+    dy_bytes = rows_of(dy_step) * dy_row;
+    dy_dst = smem + slot * SLOT + wave * 1024;
+  };
+  auto issue_dy = [&](int j) { wm8_dma16(dy_ptr, dy_bytes, dy_dst + j * 8192, dvoff[j]); };
+  auto end_dy = [&]() {
+    dy_ptr += (long long)WM8_MS * dy_row;
+    ++dy_step;
+  };
+  auto has_unit = [&](int u) { return u < UFULL || u * 512 + wave * 64 < UNITS; };        // wave-uniform
+  unsigned char* const raw = smem + 2 * SLOT;
+  unsigned udata[UMAX], uscale[UMAX];
 #pragma unroll
-    for (int j = 0; j < JMAX; ++j) {
-      const int q = j * 8 + wave;
-      if (j < JMIN || q < NI0) wm8_dma16(dy_ptr, bytes, smem + slot * SLOT + q * 1024, dvoff[j]);   // wave-uniform
-    }
-    dy_ptr += dy_step;
-    dy_left -= dy_step;
+  for (int u = 0; u < UMAX; ++u) {
+    const int id = u * 512 + tid, row = id / UPR, half = id - row * UPR, blk = (k0 >> 5) + (half >> 1);
+    udata[u] = blk < p.blocks ? (unsigned)row * xd_row + blk * 32u + (half & 1) * 16u : OOB;
+    uscale[u] = blk < p.blocks ? (unsigned)row * p.sstride + (blk & ~3) : OOB;
+  }
+  const unsigned char* xd_ptr = p.x + (long long)step_begin * WM8_MS * xd_row;
+  const unsigned char* xs_ptr = p.xs + (long long)step_begin * WM8_MS * p.sstride;
+  int x_step = step_begin;
+  auto load_x = [&](int place) {
+    const int rows = rows_of(x_step);
+    unsigned char* const dst = raw + place * RAW;
+#pragma unroll
+    for (int u = 0; u < UMAX; ++u)
+      if (has_unit(u)) {
+        wm8_dma16(xd_ptr, rows * xd_row, dst + (u * 8 + wave) * 1024, udata[u]);
+        wm8_dma4(xs_ptr, rows * p.sstride, dst + UNITS * 16 + (u * 8 + wave) * 256, uscale[u]);
+      }
+    xd_ptr += (long long)WM8_MS * xd_row;
+    xs_ptr += (long long)WM8_MS * p.sstride;
+    ++x_step;
   };
 
-  // x: a thread's unit is 16 elements of one row and their block's scale byte
-  int urow[UMAX];
+  // ---- widening: this thread's units
   unsigned udst[UMAX];
-  bool uok[UMAX];
-  long long udata[UMAX], uscale[UMAX];
+  int ubyte[UMAX];
 #pragma unroll
   for (int u = 0; u < UMAX; ++u) {
     const int id = u * 512 + tid, row = id / UPR, half = id - row * UPR;
-    const int blk = (k0 >> 5) + (half >> 1);
-    urow[u] = row;
-    uok[u] = (u < UFULL || id < WM8_MS * UPR) && blk < p.blocks;
     udst[u] = IMG0 + row * (T1 * 2) + (((2 * half) ^ wm8_swz<T1>(row)) << 4);
-    udata[u] = ((long long)row * p.blocks + blk) * 32 + (half & 1) * 16;
-    uscale[u] = (long long)row * p.sstride + blk;
+    ubyte[u] = 8 * (((k0 >> 5) + (half >> 1)) & 3);
   }
-  long long x_row = (long long)step_begin * WM8_MS;        // first row of the step to load next
-  uint4 raw[UMAX];
-  int code[UMAX];
-  auto load_x = [&]() {
-    const unsigned char* xb = p.x + x_row * p.blocks * 32;
-    const unsigned char* sb = p.xs + x_row * p.sstride;
+  uint4 xraw[UMAX];
+  unsigned xcode[UMAX];
+  auto read_raw = [&](int place) {
 #pragma unroll
     for (int u = 0; u < UMAX; ++u) {
-      raw[u] = make_uint4(0, 0, 0, 0);
-      code[u] = 0;
-      if (u >= UFULL && wave * 64 + u * 512 >= WM8_MS * UPR) continue;     // wave-uniform
-      if (uok[u] && x_row + urow[u] < p.rows) {
-        raw[u] = *reinterpret_cast<const uint4*>(xb + udata[u]);
-        code[u] = sb[uscale[u]];
+      xraw[u] = make_uint4(0, 0, 0, 0);
+      xcode[u] = 0;
+      if (has_unit(u)) {
+        xraw[u] = *reinterpret_cast<const uint4*>(raw + place * RAW + (u * 512 + tid) * 16);
+        xcode[u] = *reinterpret_cast<const unsigned*>(raw + place * RAW + UNITS * 16 + (u * 512 + tid) * 4);
       }
     }
-    x_row += WM8_MS;
   };
-  auto widen_x = [&](int slot) {
+  uint32_t wide[8];
+  float one = 0.f;
+  auto widen_begin = [&](auto unit) {
+    constexpr int u = decltype(unit)::value;
+    const int code = (int)(xcode[u] >> ubyte[u]) & 255;
+    one = code == 255 ? __uint_as_float(0x7fc00000u) : ldexpf(1.0f, code - 133);
+  };
+  auto widen_word = [&](auto unit, auto word) {            // four elements
+    constexpr int u = decltype(unit)::value, i = decltype(word)::value;
+    const unsigned w = i == 0 ? xraw[u].x : i == 1 ? xraw[u].y : i == 2 ? xraw[u].z : xraw[u].w;
+    float v[4];
 #pragma unroll
-    for (int u = 0; u < UMAX; ++u) {
-      if (u >= UFULL && wave * 64 + u * 512 >= WM8_MS * UPR) continue;
-      const float step = code[u] == 255 ? __uint_as_float(0x7fc00000u) : ldexpf(1.0f, code[u] - 133);
-      const unsigned w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
-      uint32_t o[8];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        float v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = (float)((int)(w[q] << (24 - 8 * e)) >> 24) * step;
-        o[2 * q] = pack_bf16x2(v[0], v[1]);
-        o[2 * q + 1] = pack_bf16x2(v[2], v[3]);
-      }
-      uint4* d = reinterpret_cast<uint4*>(smem + slot * SLOT + udst[u]);
-      d[0] = make_uint4(o[0], o[1], o[2], o[3]);
-      d[1] = make_uint4(o[4], o[5], o[6], o[7]);
+    for (int e = 0; e < 4; ++e) v[e] = (float)((int)(w << (24 - 8 * e)) >> 24) * one;
+    wide[2 * i] = pack_bf16x2(v[0], v[1]);
+    wide[2 * i + 1] = pack_bf16x2(v[2], v[3]);
+  };
+  auto widen = [&](auto unit) {
+    widen_begin(unit);
+    [&]<int... I>(std::integer_sequence<int, I...>) { (widen_word(unit, std::integral_constant<int, I>{}), ...); }(std::make_integer_sequence<int, 4>{});
+  };
+  auto write_wide = [&](auto unit, int slot) {
+    constexpr int u = decltype(unit)::value;
+    uint4* d = reinterpret_cast<uint4*>(smem + slot * SLOT + udst[u]);
+    if (has_unit(u)) {
+      d[0] = make_uint4(wide[0], wide[1], wide[2], wide[3]);
+      d[1] = make_uint4(wide[4], wide[5], wide[6], wide[7]);
     }
   };
+  using First = std::integral_constant<int, 0>;
+  using Last = std::integral_constant<int, UMAX - 1>;
 
   f32x4_t acc[F0][F1];
 #pragma unroll
@@ -152,101 +222,126 @@ linear_wgrad_mx8_kernel(const WgradMx8Params p) {
 #pragma unroll
     for (int j = 0; j < F1; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
-  // transposed fragments: lane -> row 4 fq + tq (and 16 further down, where the swizzle is the same), chunk 2 ct + (tp >> 1), half tp & 1
+  // transposed fragments: lane -> row 4 fq + tq (and 16, 32, 48 further down, where the swizzle is the same), chunk 2 ct + (tp >> 1),
+  // half tp & 1
   const int fr = lane & 15, fq = lane >> 4, tq = fr >> 2, tp = fr & 3;
   const int frow = 4 * fq + tq;
   const unsigned lds_base = (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
-  unsigned off0[F0], off1[F1];
+  constexpr int NO0 = wm8_distinct<T0, F0>(), NO1 = wm8_distinct<T1, F1>();
+  unsigned off0[NO0], off1[NO1];
 #pragma unroll
-  for (int i = 0; i < F0; ++i)
-    off0[i] = frow * (T0 * 2) + (((2 * (w0 * F0 + i) + (tp >> 1)) ^ wm8_swz<T0>(frow)) << 4) + ((tp & 1) << 3);
+  for (int i = 0; i < NO0; ++i)
+    off0[i] = lds_base + frow * (T0 * 2) + (((2 * (w0 * F0 + i) + (tp >> 1)) ^ wm8_swz<T0>(frow)) << 4) + ((tp & 1) << 3);
 #pragma unroll
-  for (int j = 0; j < F1; ++j)
-    off1[j] = IMG0 + frow * (T1 * 2) + (((2 * (w1 * F1 + j) + (tp >> 1)) ^ wm8_swz<T1>(frow)) << 4) + ((tp & 1) << 3);
+  for (int j = 0; j < NO1; ++j)
+    off1[j] = lds_base + IMG0 + frow * (T1 * 2) + (((2 * (w1 * F1 + j) + (tp >> 1)) ^ wm8_swz<T1>(frow)) << 4) + ((tp & 1) << 3);
 
+  struct Frags { bf16x4_t lo0[F0], hi0[F0], lo1[F1], hi1[F1]; };
+  auto read_fragments = [&](Frags& f, int slot, auto block) {
+    constexpr int B = decltype(block)::value;
+    const unsigned sbase = slot * SLOT;
+    [&]<int... I>(std::integer_sequence<int, I...>) {
+      ([&] {
+        constexpr int i = I;
+        tr_read<i / NO0 * (NO0 * 32) + B * 32 * T0 * 2>(f.lo0[i], sbase + off0[i % NO0]);
+        tr_read<i / NO0 * (NO0 * 32) + (B * 32 + 16) * T0 * 2>(f.hi0[i], sbase + off0[i % NO0]);
+      }(), ...);
+    }(std::make_integer_sequence<int, F0>{});
+    [&]<int... J>(std::integer_sequence<int, J...>) {
+      ([&] {
+        constexpr int j = J;
+        tr_read<j / NO1 * (NO1 * 32) + B * 32 * T1 * 2>(f.lo1[j], sbase + off1[j % NO1]);
+        tr_read<j / NO1 * (NO1 * 32) + (B * 32 + 16) * T1 * 2>(f.hi1[j], sbase + off1[j % NO1]);
+      }(), ...);
+    }(std::make_integer_sequence<int, F1>{});
+  };
+  auto here = [&](Frags& f) {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < F0; ++i) asm volatile("" : "+v"(f.lo0[i]), "+v"(f.hi0[i]));   // no use of a fragment moves above the wait
+#pragma unroll
+    for (int j = 0; j < F1; ++j) asm volatile("" : "+v"(f.lo1[j]), "+v"(f.hi1[j]));
+  };
+  auto multiply = [&](const Frags& f) {
+    auto join = [](const bf16x4_t& lo, const bf16x4_t& hi) {
+      return bf16x8_t{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    };
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int i = 0; i < F0; ++i)
+#pragma unroll
+      for (int j = 0; j < F1; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(join(f.lo1[j], f.hi1[j]), join(f.lo0[i], f.hi0[i]), acc[i][j], 0, 0, 0);
+    __builtin_amdgcn_s_setprio(0);
+    __builtin_amdgcn_sched_barrier(0);
+  };
   if (nsteps > 0) {
-    // In memory order: x(s + 1) in registers, then dY(s + 1) to LDS -- a wait that leaves only this wave's youngest DMA batch in flight
-    // has dY(s) in LDS and x(s + 1) in registers, whether or not the x loads were issued.
-    load_x();
-    stage_dy(0);
-    widen_x(0);
-    if (nsteps > 1) { load_x(); stage_dy(1); }
-    const bool three = JMAX > JMIN && (JMIN * 8 + wave) < NI0;
-    int slot = 0;
-    for (int s = 0; s < nsteps; ++s) {
-      if (s + 1 < nsteps) {
-        if (three) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(JMAX) : "memory");
-        else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(JMIN) : "memory");
-      } else {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      }
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // this wave's widened x(s) is in LDS
-      __builtin_amdgcn_s_barrier();                        // everybody's is; the slot of step s - 1 is free
-      asm volatile("" ::: "memory");
-      const unsigned sbase = lds_base + slot * SLOT;
-      const int next = slot == 2 ? 0 : slot + 1, after = next == 2 ? 0 : next + 1;
-      bf16x4_t lo0[F0], hi0[F0], lo1[F1], hi1[F1];
-      constexpr bool OUT0 = F0 >= F1;                      // the longer fragment list is the outer loop of the MFMAs
-      constexpr int NOUT = OUT0 ? F0 : F1;
-      auto read0 = [&](int i) {
-        asm volatile("ds_read_b64_tr_b16 %0, %1" : "=v"(lo0[i]) : "v"(sbase + off0[i]) : "memory");
-        asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2" : "=v"(hi0[i]) : "v"(sbase + off0[i]), "n"(16 * T0 * 2) : "memory");
-      };
-      auto read1 = [&](int j) {
-        asm volatile("ds_read_b64_tr_b16 %0, %1" : "=v"(lo1[j]) : "v"(sbase + off1[j]) : "memory");
-        asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2" : "=v"(hi1[j]) : "v"(sbase + off1[j]), "n"(16 * T1 * 2) : "memory");
-      };
-      if constexpr (OUT0) {
-#pragma unroll
-        for (int j = 0; j < F1; ++j) read1(j);
-#pragma unroll
-        for (int i = 0; i < F0; ++i) read0(i);
-      } else {
-#pragma unroll
-        for (int i = 0; i < F0; ++i) read0(i);
-#pragma unroll
-        for (int j = 0; j < F1; ++j) read1(j);
-      }
+    auto arrive = [&]() {                                  // what this wave loaded and wrote is there, and then everybody's is
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    load_x(0);
+    begin_dy(0);
 #pragma unroll
-      for (int i = 0; i < F0; ++i) asm volatile("" : "+v"(lo0[i]), "+v"(hi0[i]));   // no use of a fragment moves above the wait
+    for (int j = 0; j < ND; ++j) issue_dy(j);
+    end_dy();
+    if (nsteps > 1) load_x(1);
+    arrive();
+    read_raw(0);
+    widen(First{});
+    write_wide(First{}, 0);
+    if constexpr (UMAX > 1) { widen(Last{}); write_wide(Last{}, 0); }
+    Frags f;
+    auto next_x = [&](int slot) {
+      widen(First{});
+      write_wide(First{}, slot);
+      if constexpr (UMAX > 1) { widen(Last{}); write_wide(Last{}, slot); }
+    };
+    for (int s = 0; s < nsteps; ++s) {
+      // Behind the barrier dY(s) and the widened x(s) are in slot s & 1, the stored x(s + 1) is in place (s + 1) & 1, and nobody reads
+      // slot (s + 1) & 1 or place s & 1 any more.  The plain LDS reads come before the first load: the compiler drains a wave's loads in
+      // front of one.
+      arrive();
+      const int cur = s & 1, next = cur ^ 1;
+      const bool more = s + 1 < nsteps;
+      read_raw(next);
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+      if (more) {
+        begin_dy(next);
 #pragma unroll
-      for (int j = 0; j < F1; ++j) asm volatile("" : "+v"(lo1[j]), "+v"(hi1[j]));
-      if (s + 1 < nsteps) widen_x(next);
-      if (s + 2 < nsteps) { load_x(); stage_dy(after); }
-      auto join = [](const bf16x4_t& lo, const bf16x4_t& hi) {
-        return bf16x8_t{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-      };
-#pragma unroll
-      for (int g = 0; g < NOUT; ++g) {
-        if constexpr (OUT0) {
-#pragma unroll
-          for (int j = 0; j < F1; ++j) acc[g][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(join(lo0[g], hi0[g]), join(lo1[j], hi1[j]), acc[g][j], 0, 0, 0);
-        } else {
-#pragma unroll
-          for (int i = 0; i < F0; ++i) acc[i][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(join(lo0[i], hi0[i]), join(lo1[g], hi1[g]), acc[i][g], 0, 0, 0);
-        }
+        for (int j = 0; j < ND; ++j) issue_dy(j);
+        end_dy();
       }
-      slot = next;
+      if (s + 2 < nsteps) load_x(cur);
+      // waves 0 .. 3 widen the next x behind their MFMAs, waves 4 .. 7 -- the other wave of each SIMD -- in front of them, so that a SIMD's
+      // matrix core works for one while the other converts
+      if (wave >= 4 && more) next_x(next);
+      read_fragments(f, cur, std::integral_constant<int, 0>{});
+      here(f);
+      multiply(f);
+      read_fragments(f, cur, std::integral_constant<int, 1>{});
+      here(f);
+      multiply(f);
+      if (wave < 4 && more) next_x(next);
     }
   }
 
-  // C[row = n = 4 fq + r][column = k = fr]
-  float* out = p.out + (long long)blockIdx.y * p.n * p.k;
+  // x is the instruction's first operand: a lane has four consecutive k (rows 4 fq .. + 3 of the fragment) of one n (column fr)
+  float* out = p.out + (long long)split * p.n * p.k;
 #pragma unroll
-  for (int i = 0; i < F0; ++i)
+  for (int i = 0; i < F0; ++i) {
+    const int n = n0 + (w0 * F0 + i) * 16 + fr;
+    float* row = out + (long long)n * p.k + k0 + w1 * (T1 / W1) + fq * 4;
+    const int left = n < p.n ? p.k - (k0 + w1 * (T1 / W1) + fq * 4) : 0;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int n = n0 + (w0 * F0 + i) * 16 + fq * 4 + r;
-      if (n >= p.n) continue;
-#pragma unroll
-      for (int j = 0; j < F1; ++j) {
-        const int k = k0 + (w1 * F1 + j) * 16 + fr;
-        if (k >= p.k) continue;
-        float* d = out + (long long)n * p.k + k;
-        *d = p.accumulate ? *d + acc[i][j][r] : acc[i][j][r];
-      }
-    }
+    for (int j = 0; j < F1; ++j) wm8_store(row + j * 16, left - j * 16, acc[i][j], p.vec_out, p.accumulate);
+  }
 }
 
 // dw (+)= the partial tiles, in order
@@ -259,13 +354,13 @@ wgrad_mx8_fold_kernel(const float* __restrict__ partial, float* __restrict__ dw,
   dw[i] = v;
 }
 
-// Tile shape with the least padded work (channel counts of this model family are multiples of 320), then enough splits of the rows for
-// one workgroup on every CU, at least 16 steps each
+// Tile shape: least padded work (channel counts of this model family are multiples of 320), then the larger one.  Enough splits of the
+// rows for one workgroup on every CU but no second round, at least 4 steps each.
 static int wgrad_mx8_plan(long long rows, int n, int k, WgradMx8Params& p) {
-  static const int shapes[3][2] = {{256, 256}, {320, 256}, {256, 320}};
+  static const int shapes[4][2] = {{320, 160}, {256, 192}, {256, 160}, {256, 128}};
   long long best = -1;
   int cfg = 0;
-  for (int c = 0; c < 3; ++c) {
+  for (int c = 0; c < 4; ++c) {
     const long long tn = (n + shapes[c][0] - 1) / shapes[c][0], tk = (k + shapes[c][1] - 1) / shapes[c][1];
     const long long padded = tn * shapes[c][0] * tk * shapes[c][1];
     if (best < 0 || padded < best) { best = padded; cfg = c; p.tiles_n = (int)tn; p.tiles_k = (int)tk; }
@@ -273,7 +368,7 @@ static int wgrad_mx8_plan(long long rows, int n, int k, WgradMx8Params& p) {
   const int steps = (int)((rows + WM8_MS - 1) / WM8_MS);
   const long long tiles = (long long)p.tiles_n * p.tiles_k;
   long long splits = tiles >= 256 ? 1 : 256 / tiles;
-  if (splits > steps / 16) splits = steps / 16;
+  if (splits > steps / 4) splits = steps / 4;
   if (splits < 1) splits = 1;
   p.steps_per_split = (int)((steps + splits - 1) / splits);
   p.splits = (steps + p.steps_per_split - 1) / p.steps_per_split;
@@ -282,7 +377,8 @@ static int wgrad_mx8_plan(long long rows, int n, int k, WgradMx8Params& p) {
 
 template <int T0, int T1, int W0, int W1>
 static int launch_wgrad_mx8(const WgradMx8Params& p, hipStream_t st) {
-  constexpr int smem = 3 * WM8_MS * (T0 + T1) * 2;
+  constexpr int smem = 2 * WM8_MS * ((T0 + T1) * 2 + (T1 / 16) * 20);
+  static_assert(smem <= 160 * 1024, "LDS");
   auto kern = linear_wgrad_mx8_kernel<T0, T1, W0, W1>;
   static bool done = false;
   if (!done) {
@@ -290,7 +386,7 @@ static int launch_wgrad_mx8(const WgradMx8Params& p, hipStream_t st) {
     if (e != hipSuccess) { set_error("ldm_linear_wgrad_mx8: hipFuncSetAttribute: %s", hipGetErrorString(e)); return LDM_EHIP; }
     done = true;
   }
-  hipLaunchKernelGGL(kern, dim3(p.tiles_n * p.tiles_k, p.splits), dim3(512), smem, st, p);
+  hipLaunchKernelGGL(kern, dim3((unsigned)(p.tiles_n * p.tiles_k * p.splits)), dim3(512), smem, st, p);
   return LDM_OK;
 }
 
@@ -312,19 +408,24 @@ extern "C" long long ldm_linear_wgrad_mx8_workspace_bytes(long long rows, int n,
 extern "C" int ldm_linear_wgrad_mx8(const void* x8, const void* x8_scale, const void* dy, float* dw, long long rows, int n, int k,
                                     int accumulate, void* workspace, long long workspace_bytes, void* stream) {
   LDM_REQUIRE(wgrad_mx8_sizes_ok(rows, n, k) && n % 8 == 0, "ldm_linear_wgrad_mx8: bad sizes (rows=%lld n=%d k=%d; n a multiple of 8)", rows, n, k);
-  LDM_REQUIRE(x8 && x8_scale && dy && dw && aligned16(x8) && aligned16(dy), "ldm_linear_wgrad_mx8: null or unaligned pointer");
+  LDM_REQUIRE(x8 && x8_scale && dy && dw && aligned16(x8) && aligned16(dy) && (reinterpret_cast<uintptr_t>(x8_scale) & 3) == 0,
+              "ldm_linear_wgrad_mx8: null or unaligned pointer");
   WgradMx8Params p;
   const int cfg = wgrad_mx8_plan(rows, n, k, p);
   const long long need = p.splits > 1 ? (long long)p.splits * n * k * 4 : 0;
   LDM_REQUIRE(need == 0 || (workspace != nullptr && aligned16(workspace) && workspace_bytes >= need),
               "ldm_linear_wgrad_mx8: workspace of %lld bytes needed (got %lld)", need, workspace_bytes);
-  LDM_REQUIRE((long long)p.tiles_n * p.tiles_k < (1LL << 31) && p.splits <= 65535, "ldm_linear_wgrad_mx8: too large");
+  LDM_REQUIRE((long long)p.tiles_n * p.tiles_k * p.splits < (1LL << 31), "ldm_linear_wgrad_mx8: too large");
   p.x = static_cast<const unsigned char*>(x8); p.xs = static_cast<const unsigned char*>(x8_scale); p.dy = static_cast<const char*>(dy);
   p.rows = rows; p.n = n; p.k = k; p.blocks = mx_blocks(k); p.sstride = mx_scale_stride(k);
   p.out = need ? static_cast<float*>(workspace) : dw;
   p.accumulate = need ? 0 : accumulate;
+  p.vec_out = k % 4 == 0 && aligned16(p.out);
   hipStream_t st = (hipStream_t)stream;
-  const int rc = cfg == 0 ? launch_wgrad_mx8<256, 256, 2, 4>(p, st) : cfg == 1 ? launch_wgrad_mx8<320, 256, 2, 4>(p, st) : launch_wgrad_mx8<256, 320, 4, 2>(p, st);
+  const int rc = cfg == 0   ? launch_wgrad_mx8<320, 160, 4, 2>(p, st)
+                 : cfg == 1 ? launch_wgrad_mx8<256, 192, 4, 2>(p, st)
+                 : cfg == 2 ? launch_wgrad_mx8<256, 160, 4, 2>(p, st)
+                            : launch_wgrad_mx8<256, 128, 4, 2>(p, st);
   if (rc) return rc;
   LDM_HIP_CHECK_LAUNCH("ldm_linear_wgrad_mx8");
   if (need) {

@@ -187,7 +187,10 @@ static inline void raw_ptr_buffer_load_lds(rsrc_t rs, void* lds, int size, unsig
   dma_to_lds(dst, chk + size <= rs.bytes ? rs.base + off : nullptr, size);
 }
 typedef unsigned u32x4_emu __attribute__((ext_vector_type(4)));
+// A load into registers lands at once here, but it has its place in the order that s_waitcnt vmcnt(n) counts
+static inline void count_load() { dma_to_lds(nullptr, nullptr, 0); }
 static inline u32x4_emu raw_buffer_load_b128(rsrc_t rs, int voff, int soff, int) {
+  count_load();
   const unsigned long long chk = (unsigned long long)(unsigned)voff + (soff_checked() ? (unsigned)soff : 0u);
   const unsigned long long off = (unsigned long long)(unsigned)voff + (unsigned)soff;
   u32x4_emu r{0, 0, 0, 0};
@@ -195,6 +198,7 @@ static inline u32x4_emu raw_buffer_load_b128(rsrc_t rs, int voff, int soff, int)
   return r;
 }
 static inline unsigned raw_buffer_load_b32(rsrc_t rs, int voff, int soff, int) {
+  count_load();
   const unsigned long long chk = (unsigned long long)(unsigned)voff + (soff_checked() ? (unsigned)soff : 0u);
   const unsigned long long off = (unsigned long long)(unsigned)voff + (unsigned)soff;
   unsigned r = 0;
