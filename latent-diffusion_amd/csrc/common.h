@@ -94,6 +94,15 @@ __device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
   *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
 }
 
+// the same at any element alignment: one 16-byte access each (global memory takes them unaligned), not eight small ones
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4_any_t;
+typedef u32x4_any_t __attribute__((aligned(2))) u32x4_a2_t;
+__device__ __forceinline__ uint4 load16_any(const void* p) {
+  const u32x4_any_t r = *reinterpret_cast<const u32x4_a2_t*>(p);
+  return make_uint4(r[0], r[1], r[2], r[3]);
+}
+__device__ __forceinline__ void store16_any(void* p, uint4 v) { *reinterpret_cast<u32x4_a2_t*>(p) = u32x4_any_t{v.x, v.y, v.z, v.w}; }
+
 __device__ __forceinline__ float silu_f(float x) { return x / (1.0f + __expf(-x)); }
 __device__ __forceinline__ float gelu_erf_f(float x) { return 0.5f * x * (1.0f + erff(x * 0.70710678118654752440f)); }
 

@@ -106,6 +106,30 @@ __device__ __forceinline__ void decode4(unsigned w, int code, float (&v)[8]) {
   v[0] = a[0]; v[1] = a[1]; v[2] = b[0]; v[3] = b[1]; v[4] = c[0]; v[5] = c[1]; v[6] = d[0]; v[7] = d[1];
 }
 
+// 8 floats of a row that may start at any element
+__device__ __forceinline__ void load8_any(const bf16_t* p, float (&v)[8]) {
+  const uint4 r = load16_any(p);
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(w[i] << 16);
+    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void load8_any(const float* p, float (&v)[8]) {
+  const uint4 a = load16_any(p), b = load16_any(p + 4);
+  const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i]);
+}
+__device__ __forceinline__ void store8_any(bf16_t* p, const float (&v)[8]) {
+  store16_any(p, make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])));
+}
+__device__ __forceinline__ void store8_any(float* p, const float (&v)[8]) {
+  store16_any(p, make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])));
+  store16_any(p + 4, make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7])));
+}
+
 // ---------------------------------------------------------------------------------------------------------------- quantise
 constexpr int MX_U = 4;        // chunks a thread has in flight
 
@@ -121,7 +145,7 @@ struct MxParams {
 };
 
 // Chunks are counted over rows filled up to whole scale words, so the threads of a row's padding write its padding bytes.
-template <typename T, int FMT, bool VEC>
+template <typename T, int FMT>
 __global__ void __launch_bounds__(256)
 mx_quantize_kernel(const MxParams p) {
   float v[MX_U][8];
@@ -137,8 +161,8 @@ mx_quantize_kernel(const MxParams p) {
     for (int e = 0; e < 8; ++e) v[u][e] = 0.f;
     if (idx >= p.total || col >= p.cols) continue;
     const T* src = static_cast<const T*>(p.src) + (long long)row[u] * p.ld + col;
-    if (VEC && col + 8 <= p.cols) {
-      load8(src, v[u]);
+    if (col + 8 <= p.cols) {
+      load8_any(src, v[u]);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
@@ -161,7 +185,7 @@ mx_quantize_kernel(const MxParams p) {
   }
 }
 
-template <typename T, int FMT, bool VEC>
+template <typename T, int FMT>
 __global__ void __launch_bounds__(256)
 mx_dequantize_kernel(const MxParams p) {
   uint2 w[MX_U];
@@ -190,8 +214,8 @@ mx_dequantize_kernel(const MxParams p) {
     else decode8(w[u], step8(code[u]), v);
     const int col = (int)ch[u] * 8;
     T* dst = static_cast<T*>(p.dst) + (long long)row[u] * p.ld + col;
-    if (VEC && col + 8 <= p.cols) {
-      store8(dst, v);
+    if (col + 8 <= p.cols) {
+      store8_any(dst, v);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
@@ -383,16 +407,12 @@ glu_bwd_mx8_kernel(const GluMx8Params p) {
 static long long rows_a_launch(long long chunks_a_row) { return 0x7ff00000LL / chunks_a_row; }
 
 template <typename T, int FMT>
-static void launch_quantize(const MxParams& p, bool vec, hipStream_t st) {
-  const dim3 grid((p.total + 256u * MX_U - 1) / (256u * MX_U));
-  if (vec) hipLaunchKernelGGL((mx_quantize_kernel<T, FMT, true>), grid, dim3(256), 0, st, p);
-  else hipLaunchKernelGGL((mx_quantize_kernel<T, FMT, false>), grid, dim3(256), 0, st, p);
+static void launch_quantize(const MxParams& p, hipStream_t st) {
+  hipLaunchKernelGGL((mx_quantize_kernel<T, FMT>), dim3((p.total + 256u * MX_U - 1) / (256u * MX_U)), dim3(256), 0, st, p);
 }
 template <typename T, int FMT>
-static void launch_dequantize(const MxParams& p, bool vec, hipStream_t st) {
-  const dim3 grid((p.total + 256u * MX_U - 1) / (256u * MX_U));
-  if (vec) hipLaunchKernelGGL((mx_dequantize_kernel<T, FMT, true>), grid, dim3(256), 0, st, p);
-  else hipLaunchKernelGGL((mx_dequantize_kernel<T, FMT, false>), grid, dim3(256), 0, st, p);
+static void launch_dequantize(const MxParams& p, hipStream_t st) {
+  hipLaunchKernelGGL((mx_dequantize_kernel<T, FMT>), dim3((p.total + 256u * MX_U - 1) / (256u * MX_U)), dim3(256), 0, st, p);
 }
 
 }  // namespace ldm
@@ -413,7 +433,6 @@ extern "C" int ldm_mx_quantize(const void* x, int dtype, long long rows, int col
   LDM_REQUIRE(x && data && scale && aligned16(data) && (reinterpret_cast<uintptr_t>(scale) & 3) == 0 &&
                   reinterpret_cast<uintptr_t>(x) % dtype_size(dtype) == 0, "ldm_mx_quantize: null or unaligned pointer");
   const size_t es = dtype_size(dtype);
-  const bool vec = aligned16(x) && (ld * es) % 16 == 0;
   MxParams p;
   p.ld = ld; p.cols = cols; p.blocks = mx_blocks(cols); p.sstride = mx_scale_stride(cols); p.dst = nullptr;
   p.cpr = fast_div((unsigned)p.sstride * 4u);
@@ -424,8 +443,8 @@ extern "C" int ldm_mx_quantize(const void* x, int dtype, long long rows, int col
     p.data = static_cast<char*>(data) + r * p.blocks * bytes;
     p.scale = static_cast<unsigned char*>(scale) + r * p.sstride;
     p.total = (unsigned)(n * p.sstride * 4);
-    if (dtype == LDM_BF16) fmt == LDM_MX4 ? launch_quantize<bf16_t, LDM_MX4>(p, vec, (hipStream_t)stream) : launch_quantize<bf16_t, LDM_MX8>(p, vec, (hipStream_t)stream);
-    else fmt == LDM_MX4 ? launch_quantize<float, LDM_MX4>(p, vec, (hipStream_t)stream) : launch_quantize<float, LDM_MX8>(p, vec, (hipStream_t)stream);
+    if (dtype == LDM_BF16) fmt == LDM_MX4 ? launch_quantize<bf16_t, LDM_MX4>(p, (hipStream_t)stream) : launch_quantize<bf16_t, LDM_MX8>(p, (hipStream_t)stream);
+    else fmt == LDM_MX4 ? launch_quantize<float, LDM_MX4>(p, (hipStream_t)stream) : launch_quantize<float, LDM_MX8>(p, (hipStream_t)stream);
     LDM_HIP_CHECK_LAUNCH("ldm_mx_quantize");
   }
   return LDM_OK;
@@ -438,7 +457,6 @@ extern "C" int ldm_mx_dequantize(const void* data, const void* scale, int fmt, l
   LDM_REQUIRE(out && data && scale && aligned16(data) && (reinterpret_cast<uintptr_t>(scale) & 3) == 0 &&
                   reinterpret_cast<uintptr_t>(out) % dtype_size(dtype) == 0, "ldm_mx_dequantize: null or unaligned pointer");
   const size_t es = dtype_size(dtype);
-  const bool vec = aligned16(out) && (ld * es) % 16 == 0;
   MxParams p;
   p.ld = ld; p.cols = cols; p.blocks = mx_blocks(cols); p.sstride = mx_scale_stride(cols); p.src = nullptr;
   const int chunks = (cols + 7) / 8;
@@ -450,8 +468,8 @@ extern "C" int ldm_mx_dequantize(const void* data, const void* scale, int fmt, l
     p.data = const_cast<char*>(static_cast<const char*>(data) + r * p.blocks * bytes);
     p.scale = const_cast<unsigned char*>(static_cast<const unsigned char*>(scale) + r * p.sstride);
     p.total = (unsigned)(n * chunks);
-    if (dtype == LDM_BF16) fmt == LDM_MX4 ? launch_dequantize<bf16_t, LDM_MX4>(p, vec, (hipStream_t)stream) : launch_dequantize<bf16_t, LDM_MX8>(p, vec, (hipStream_t)stream);
-    else fmt == LDM_MX4 ? launch_dequantize<float, LDM_MX4>(p, vec, (hipStream_t)stream) : launch_dequantize<float, LDM_MX8>(p, vec, (hipStream_t)stream);
+    if (dtype == LDM_BF16) fmt == LDM_MX4 ? launch_dequantize<bf16_t, LDM_MX4>(p, (hipStream_t)stream) : launch_dequantize<bf16_t, LDM_MX8>(p, (hipStream_t)stream);
+    else fmt == LDM_MX4 ? launch_dequantize<float, LDM_MX4>(p, (hipStream_t)stream) : launch_dequantize<float, LDM_MX8>(p, (hipStream_t)stream);
     LDM_HIP_CHECK_LAUNCH("ldm_mx_dequantize");
   }
   return LDM_OK;

@@ -30,7 +30,7 @@ struct Mx4Params {
   int n, k, blocks, sstride;   // N, K, blocks and scale bytes a row
   int nk;                      // steps of 128 columns
   int tiles_m, tiles_n;
-  int vec_out;                 // 16-byte stores of the output are legal
+  int vec_out;                 // four neighbours of a row can be stored at once (few rows)
 };
 
 // bijective XCD remap: workgroups b and b + 8 share an XCD; every XCD gets a contiguous run of tiles
@@ -51,23 +51,46 @@ __device__ __forceinline__ void mx_dma4(const void* base, unsigned bytes, unsign
   __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)lds, 4, voff, soff, 0, 0);
 }
 
-// Tile of BM (rows of x) x BN (rows of w) by WM x WN waves, 128 columns (64 bytes a row) a step, S slots of LDS: the LDS-DMA of S - 1
-// steps is in flight.  16-byte chunks of a row are XOR-swizzled by (row >> 1) & 3 (the DMA writes lane-linear, so the swizzle is
-// applied to the lane's SOURCE chunk and again on the read): eight consecutive rows then lie in eight different 16-byte
-// columns of the 128-byte LDS line.  A chunk IS a block, so chunks past the last block are fetched from beyond the descriptor's end
-// (zeros), and rows past the end likewise.
+// LDS reads that the caller waits for: around reads of its own the compiler would wait for every LDS-DMA in flight, also those of
+// the steps ahead.
+template <int OFF>
+__device__ __forceinline__ void lds_read16(i32x4_t& v, unsigned addr) {
+  asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(v) : "v"(addr), "n"(OFF) : "memory");
+}
+template <int OFF>
+__device__ __forceinline__ void lds_read4(int& v, unsigned addr) {
+  asm volatile("ds_read_b32 %0, %1 offset:%2" : "=v"(v) : "v"(addr), "n"(OFF) : "memory");
+}
+template <bool MX, int H>
+__device__ __forceinline__ void mx_mfma(f32x16_t& c, i32x4_t a, i32x4_t b, int sa, int sb) {
+  if constexpr (MX)
+    c = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(i32x8_t{a[0], a[1], a[2], a[3], 0, 0, 0, 0}, i32x8_t{b[0], b[1], b[2], b[3], 0, 0, 0, 0}, c, 4, 4,
+                                                        2 * H, sa, 2 * H, sb);
+  else
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+}
+
+// Tile of BM (rows of x) x BN (rows of w) by WM x WN waves; a step is 64 bytes of every row (MX: 128 columns of mx4, four blocks; else 32
+// columns of bf16), S slots of LDS.  16-byte chunks of a row are XOR-swizzled by (row >> 1) & 3 (the DMA writes lane-linear, so the
+// swizzle is applied to the lane's SOURCE chunk and again on the read): eight consecutive rows then lie in eight different 16-byte
+// columns of the 128-byte LDS line.  A chunk is what a lane gives one matrix instruction -- a block, or 8 columns of bf16 -- so
+// chunks past the end of a row are fetched from beyond the descriptor's end (zeros), and rows past the end likewise.
+//
+// Each step has two halves, one matrix instruction deep; the registers of one are read while the other multiplies:
+//   multiply half 0 | read half 1;  wait for the next step's DMA, barrier;  multiply half 1 | refill the slot, read the next half 0
+// so the matrix cores wait for nothing but the skew at the one barrier a step.
 //
 // Scales: one 32-bit word a row and step.  From four steps on, 16 bytes (four steps) a row at a time in one DMA instruction, the last
 // ones ending with the row (a fetch never passes its row); with fewer steps word by word, once.
-template <int BM, int BN, int WM, int WN, int S, typename OUT>
-__global__ void __launch_bounds__(64 * WM * WN, WM * WN == 8 ? 2 : 2)
+template <int BM, int BN, int WM, int WN, int S, bool MX, typename OUT>
+__global__ void __launch_bounds__(64 * WM * WN, 2)
 mx4_gemm_kernel(const Mx4Params p) {
   constexpr int NT = 64 * WM * WN, ROWS = BM + BN;
   constexpr int IT = ROWS * 4 / NT;                        // tile DMA instructions of a wave a step
   constexpr int SIT = ROWS / NT;                           // scale DMA instructions of a wave (16 bytes a row)
-  static_assert(ROWS * 4 % NT == 0 && ROWS % NT == 0 && BM % 64 == 0, "tile / threads mismatch");
+  static_assert(BM * 4 % NT == 0 && BN * 4 % NT == 0 && ROWS % NT == 0 && BM % 64 == 0, "tile / threads mismatch");
   constexpr int STAGE = ROWS * 64;
-  constexpr int SCALES = ROWS * 16;                        // one group of four steps
+  constexpr int SCALES = MX ? ROWS * 16 : 0;               // one group of four steps
   constexpr int WTM = BM / WM, WTN = BN / WN, MI = WTM / 32, NI = WTN / 32;
   constexpr unsigned OOB = 0x80000000u;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -78,14 +101,15 @@ mx4_gemm_kernel(const Mx4Params p) {
   const int fr = lane & 31, fh = lane >> 5;
 
   const int tile = mx_xcd_remap(blockIdx.x, gridDim.x);
-  // bands of 8 tile rows walked column by column: the tiles in flight on one XCD share their operands in its L2
-  const int band = 8 * p.tiles_n, g8 = tile / band, in = tile - g8 * band;
-  const int brows = min(p.tiles_m - g8 * 8, 8);
-  const int tn = in / brows, tm = g8 * 8 + (in - tn * brows);
+  // bands of 4 tile rows walked column by column: the tiles in flight on one XCD share their operands in its L2 (bands of 8: 3 % slower
+  // at 8192 x 8192 x 8192)
+  const int band = 4 * p.tiles_n, g4 = tile / band, in = tile - g4 * band;
+  const int brows = min(p.tiles_m - g4 * 4, 4);
+  const int tn = in / brows, tm = g4 * 4 + (in - tn * brows);
   const long long m0 = (long long)tm * BM;
   const int n0 = tn * BN;
 
-  const int rb = p.blocks * 16;
+  const int rb = MX ? p.blocks * 16 : p.k * 2, chunks = rb >> 4;
   const int mrows = (int)min((long long)BM, p.rows - m0), nrows = min(BN, p.n - n0);
   const unsigned char* xbase = p.x + m0 * rb;
   const unsigned char* wbase = p.w + (long long)n0 * rb;
@@ -94,15 +118,14 @@ mx4_gemm_kernel(const Mx4Params p) {
   const unsigned xbytes = (unsigned)mrows * rb, wbytes = (unsigned)nrows * rb;
   const unsigned xsbytes = (unsigned)mrows * p.sstride, wsbytes = (unsigned)nrows * p.sstride;
 
-
   // lane's part of tile instruction `it`: chunk q = it * NT + tid of the stage image (x rows, then w rows; four chunks a row)
   unsigned voff[IT];
-  int chunk[IT];
+  const int chunk = (tid & 3) ^ ((tid >> 3) & 3);          // NT / 4 rows on, the swizzle is the same
+  static_assert(NT / 4 % 8 == 0, "swizzle period");
 #pragma unroll
   for (int it = 0; it < IT; ++it) {
     const int row = (it * NT + tid) >> 2;
-    chunk[it] = (tid & 3) ^ ((row >> 1) & 3);
-    voff[it] = (unsigned)(row < BM ? row : row - BM) * rb + chunk[it] * 16;
+    voff[it] = (unsigned)(row < BM ? row : row - BM) * rb + chunk * 16;
   }
   const int nk = p.nk;
   const bool word_scales = nk < 4;
@@ -130,16 +153,17 @@ mx4_gemm_kernel(const Mx4Params p) {
       }
     }
   };
+  // a step past the last one is fetched like any other (zeros, into a slot that nobody reads): the loop needs no case for its end
   auto stage = [&](int kt) {
-    if ((kt & 3) == 0) stage_scales(kt >> 2);
-    unsigned char* dst = smem + (kt % S) * STAGE;
-    const bool tail = kt == nk - 1;
+    if constexpr (MX)
+      if ((kt & 3) == 0 && kt < nk) stage_scales(kt >> 2);
+    unsigned char* dst = smem + (kt % S) * STAGE + wave * 1024;
+    const bool past = kt * 4 + chunk >= chunks;
 #pragma unroll
-    for (int it = 0; it < IT; ++it) {
-      const int q0 = it * NT + wave * 64;                  // the instruction's first chunk: 16 whole rows, all of one operand
-      const unsigned vo = tail && kt * 4 + chunk[it] >= p.blocks ? OOB : voff[it];
-      if (q0 < BM * 4) mx_dma16(xbase, xbytes, dst + q0 * 16, vo, kt * 64);
-      else mx_dma16(wbase, wbytes, dst + q0 * 16, vo, kt * 64);
+    for (int it = 0; it < IT; ++it) {                      // 16 whole rows a wave and instruction, all of one operand
+      const unsigned vo = past ? OOB : voff[it];
+      if (it * NT < BM * 4) mx_dma16(xbase, xbytes, dst + it * NT * 16, vo, kt * 64);
+      else mx_dma16(wbase, wbytes, dst + it * NT * 16, vo, kt * 64);
     }
   };
 
@@ -151,55 +175,92 @@ mx4_gemm_kernel(const Mx4Params p) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 
-  auto compute = [&](int kt) {
-    const unsigned char* img = smem + (kt % S) * STAGE;
-    const int g = kt >> 2, word = kt - group_first(g);
-    const unsigned char* sc = scales + (g & 1) * SCALES + word * (word_scales ? ROWS * 4 : 4);
-    const int sstep = word_scales ? 4 : 16;
-    // byte 0: this half's block of the step's first 64 columns, byte 2: of the second
-    int sx[MI], sw[NI];
+  // fragments of the two halves; scales of this step (shifted: byte 0 this lane's block of half 0, byte 2 of half 1) and of the next
+  i32x4_t xf[2][MI], wf[2][NI];
+  int sx[MI], sw[NI], nsx[MI], nsw[NI];
 #pragma unroll
-    for (int i = 0; i < MI; ++i) sx[i] = (int)(*reinterpret_cast<const unsigned*>(sc + (wm * WTM + i * 32 + fr) * sstep) >> (8 * fh));
+  for (int i = 0; i < MI; ++i) sx[i] = nsx[i] = 0;
 #pragma unroll
-    for (int j = 0; j < NI; ++j) sw[j] = (int)(*reinterpret_cast<const unsigned*>(sc + (BM + wn * WTN + j * 32 + fr) * sstep) >> (8 * fh));
-    [&]<int... HI>(std::integer_sequence<int, HI...>) {
-      ([&] {
-        constexpr int H = HI;
-        i32x8_t xf[MI], wf[NI];
-#pragma unroll
-        for (int i = 0; i < MI; ++i) {
-          const int row = wm * WTM + i * 32 + fr;
-          xf[i] = mx4_operand(*reinterpret_cast<const uint4*>(img + row * 64 + (((2 * H + fh) ^ ((row >> 1) & 3)) << 4)));
-        }
-#pragma unroll
-        for (int j = 0; j < NI; ++j) {
-          const int row = BM + wn * WTN + j * 32 + fr;
-          wf[j] = mx4_operand(*reinterpret_cast<const uint4*>(img + row * 64 + (((2 * H + fh) ^ ((row >> 1) & 3)) << 4)));
-        }
-#pragma unroll
-        for (int i = 0; i < MI; ++i)
-#pragma unroll
-          for (int j = 0; j < NI; ++j)
-            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[j], xf[i], acc[i][j], 4, 4, 2 * H, sw[j], 2 * H, sx[i]);
-      }(), ...);
-    }(std::integer_sequence<int, 0, 1>{});
-  };
+  for (int j = 0; j < NI; ++j) sw[j] = nsw[j] = 0;
+  const unsigned lds = (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
+  const int swz = (fr >> 1) & 3;
+  const unsigned xaddr = lds + (wm * WTM + fr) * 64 + ((fh ^ swz) << 4), waddr = lds + (BM + wn * WTN + fr) * 64 + ((fh ^ swz) << 4);
+  const int sstep = word_scales ? 4 : 16;
+  const unsigned xsaddr = lds + S * STAGE + (wm * WTM + fr) * sstep, wsaddr = lds + S * STAGE + (BM + wn * WTN + fr) * sstep;
 
-  // one barrier a step: wait until this wave's DMA of step kt has landed (that of the S - 2 steps behind it may be in flight; a scale
-  // fetch among them only makes the wait stricter), barrier, refill the slot of step kt - 1, multiply
+  // q-th read of half H of the step whose image starts at `slot`: the scale words come with half 0
+  constexpr int READS = MI + NI;
+  static_assert(READS <= MI * NI, "one read behind each instruction");
+  auto read = [&]<int H, int Q>(std::integral_constant<int, H>, std::integral_constant<int, Q>, unsigned slot) {
+    constexpr int i = Q < MI ? Q : 0, j = Q < MI ? 0 : Q - MI;
+    if constexpr (Q < MI) lds_read16<i * 2048>(xf[H][i], (xaddr ^ (H * 32)) + slot);
+    else lds_read16<j * 2048>(wf[H][j], (waddr ^ (H * 32)) + slot);
+  };
+  auto read_scales = [&](int kt) {
+    if constexpr (MX) {
+      const int g = kt >> 2, word = kt - group_first(g);
+      const unsigned o = (g & 1) * SCALES + word * (word_scales ? ROWS * 4 : 4);
+      const unsigned step = 32 * sstep;
 #pragma unroll
-  for (int s = 0; s < S - 1; ++s)
-    if (s < nk) stage(s);
+      for (int i = 0; i < MI; ++i) lds_read4<0>(nsx[i], xsaddr + o + i * step);
+#pragma unroll
+      for (int j = 0; j < NI; ++j) lds_read4<0>(nsw[j], wsaddr + o + j * step);
+    }
+  };
+  auto landed = [&]<int H>(std::integral_constant<int, H>) {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < MI; ++i) asm volatile("" : "+v"(xf[H][i]));   // no use moves above the wait
+#pragma unroll
+    for (int j = 0; j < NI; ++j) asm volatile("" : "+v"(wf[H][j]));
+    if constexpr (MX && H == 0) {
+#pragma unroll
+      for (int i = 0; i < MI; ++i) { asm volatile("" : "+v"(nsx[i])); sx[i] = (int)((unsigned)nsx[i] >> (8 * fh)); }
+#pragma unroll
+      for (int j = 0; j < NI; ++j) { asm volatile("" : "+v"(nsw[j])); sw[j] = (int)((unsigned)nsw[j] >> (8 * fh)); }
+    }
+  };
+  // half H of this step on the matrix cores; behind each of the first instructions a read of the other half (of `slot`)
+  auto multiply = [&]<int H>(std::integral_constant<int, H>, unsigned slot) {
+    [&]<int... Q>(std::integer_sequence<int, Q...>) {
+      ([&] {
+        constexpr int q = Q, i = q / NI, j = q % NI;
+        mx_mfma<MX, H>(acc[i][j], wf[H][j], xf[H][i], sw[j], sx[i]);
+        if constexpr (q < READS) read(std::integral_constant<int, 1 - H>{}, std::integral_constant<int, q>{}, slot);
+        __builtin_amdgcn_sched_barrier(0);
+      }(), ...);
+    }(std::make_integer_sequence<int, MI * NI>{});
+  };
+  // until this wave's DMA of the next step has landed; that of the S - 2 steps behind it may be in flight (a fetch of scales among them
+  // only makes the wait stricter)
+  auto dma_landed = [&] { asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 2) * IT) : "memory"); };
+  constexpr std::integral_constant<int, 0> H0{};
+  constexpr std::integral_constant<int, 1> H1{};
+
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s) stage(s);
+  dma_landed();
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  stage(S - 1);
+  read_scales(0);
+  [&]<int... Q>(std::integer_sequence<int, Q...>) {
+    (read(H0, std::integral_constant<int, Q>{}, 0u), ...);
+  }(std::make_integer_sequence<int, READS>{});
+  landed(H0);
   for (int kt = 0; kt < nk; ++kt) {
-    const int ahead = nk - 1 - kt;
-    if (ahead >= S - 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 2) * IT) : "memory");
-    else if (S > 3 && ahead == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(IT) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
+    multiply(H0, (unsigned)(kt % S) * STAGE);
+    landed(H1);
+    const int next = min(kt + 1, nk - 1);                  // behind the last step itself once more, unused
+    dma_landed();
+    __builtin_amdgcn_s_barrier();                          // every wave has read slot kt, and its part of the next step is there
     asm volatile("" ::: "memory");
-    if (kt + S - 1 < nk) stage(kt + S - 1);
-    compute(kt);
+    stage(kt + S);
+    read_scales(next);
+    multiply(H1, (unsigned)(next % S) * STAGE);
+    landed(H0);
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();                                         // the slots become the epilogue's
 
   // ---- epilogue: 32 rows of the wave's tile at a time through its own LDS, then whole 16-byte pieces of rows
@@ -208,15 +269,21 @@ mx4_gemm_kernel(const Mx4Params p) {
   static_assert(WM * WN * 32 * PITCH <= S * STAGE + 2 * SCALES, "epilogue image");
   unsigned char* const cst = smem + wave * 32 * PITCH;
   float bv[NI][4][4];
+  if (p.bias != nullptr) {
 #pragma unroll
-  for (int j = 0; j < NI; ++j)
+    for (int j = 0; j < NI; ++j)
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
+      for (int q = 0; q < 4; ++q)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int n = n0 + wn * WTN + j * 32 + 8 * q + 4 * fh + e;
-        bv[j][q][e] = p.bias != nullptr && n < p.n ? p.bias[n] : 0.f;
-      }
+        for (int e = 0; e < 4; ++e) bv[j][q][e] = p.bias[min(n0 + wn * WTN + j * 32 + 8 * q + 4 * fh + e, p.n - 1)];
+  } else {
+#pragma unroll
+    for (int j = 0; j < NI; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) bv[j][q][e] = 0.f;
+  }
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
 #pragma unroll
@@ -233,7 +300,7 @@ mx4_gemm_kernel(const Mx4Params p) {
     LDM_LOCKSTEP();
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     constexpr int PPR = WTN / EPR;                         // pieces a row
-#pragma unroll
+#pragma unroll 4
     for (int t = 0; t < 32 * PPR / 64; ++t) {
       const int piece = t * 64 + lane, r = piece / PPR, c = (piece - r * PPR) * EPR;
       const long long m = m0 + wm * WTM + i * 32 + r;
@@ -241,10 +308,11 @@ mx4_gemm_kernel(const Mx4Params p) {
       if (m >= p.rows || n >= p.n) continue;
       OUT* dst = static_cast<OUT*>(p.out) + m * p.n + n;
       const unsigned char* s = cst + r * PITCH + c * (int)sizeof(OUT);
-      if (p.vec_out) {                                     // n is a multiple of the piece: no piece passes the row
-        *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(s);
-      } else {
-        for (int e = 0; e < EPR && n + e < p.n; ++e) dst[e] = reinterpret_cast<const OUT*>(s)[e];
+      if (n + EPR <= p.n) {
+        store16_any(dst, *reinterpret_cast<const uint4*>(s));
+      } else {                                             // the end of a row
+#pragma unroll 1
+        for (int e = 0; n + e < p.n; ++e) dst[e] = reinterpret_cast<const OUT*>(s)[e];
       }
     }
     LDM_LOCKSTEP();
@@ -256,14 +324,119 @@ mx4_gemm_kernel(const Mx4Params p) {
 // 16 NF rows of w and 16 MT rows of x a workgroup; its 8 waves take every 8th step of 128 columns and add up through LDS in a fixed
 // order.  Operands go straight from memory to registers (nothing is used twice by a wave), several steps' loads at once.
 //   MX  true: x in mx4, v_mfma_scale_f32_16x16x128_f8f6f4: lane l holds row l % 16, block l / 16 of the step
-//       false: x in bf16; the lane's block of w is widened to bf16 (exact: 2 significant bits) and multiplied by
-//              v_mfma_f32_16x16x32_bf16 in four pieces.  Piece s takes columns 32 (l / 16) + 8 s .. + 7 of the step from BOTH
-//              operands: a permutation of the contraction index, which the sum does not see.
-template <bool MX, int MT, int NF, bool VEC, typename OUT>
+//       false: x in bf16, four v_mfma_f32_16x16x32_bf16 a step, one for each block.  Lane group g = l / 16 of the s-th holds columns
+//              32 s + 8 g .. + 7 of x (a row's four lanes read 64 bytes in one piece: with the lane's own block, 32 g + 8 s, every load
+//              of x touched 64 pieces of 16 bytes).  The weights are loaded 16 bytes a lane -- block g -- and turned among the four
+//              groups: dword g of group s becomes dword s of group g, a 4 x 4 transposition in four lane-swap instructions.  They are
+//              widened to bf16 (exact: 2 significant bits) two at a time by the conversion that takes the scale along.
+typedef __attribute__((ext_vector_type(2))) unsigned int u32x2_t;
+__device__ __forceinline__ void turn_groups(uint4& v) {
+  u32x2_t a = __builtin_amdgcn_permlane32_swap(v.x, v.z, false, false), b = __builtin_amdgcn_permlane32_swap(v.y, v.w, false, false);
+  const u32x2_t c = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false), d = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
+  v = make_uint4(c[0], c[1], d[0], d[1]);
+}
+
+// a lane's operands of one step
+template <bool MX, int MT, int NF>
+struct RowsStep {
+  uint4 wv[NF], xv[MT][MX ? 1 : 4];
+  unsigned wc[NF];                                         // MX: the lane's scale byte; else the step's four
+  int xc[MT];
+
+  __device__ __forceinline__ void load(const unsigned char* const (&w)[NF], const unsigned char* const (&ws)[NF], const unsigned char* const (&x)[MT],
+                                       const unsigned char* const (&xs)[MT], int kt, int fq) {
+#pragma unroll
+    for (int i = 0; i < NF; ++i) {
+      wv[i] = *reinterpret_cast<const uint4*>(w[i] + kt * 64 + fq * 16);
+      if constexpr (MX) wc[i] = ws[i][kt * 4 + fq];
+      else wc[i] = *reinterpret_cast<const unsigned*>(ws[i] + kt * 4);
+    }
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+      if constexpr (MX) {
+        xv[j][0] = *reinterpret_cast<const uint4*>(x[j] + kt * 64 + fq * 16);
+        xc[j] = xs[j][kt * 4 + fq];
+      } else {
+#pragma unroll
+        for (int s = 0; s < 4; ++s) xv[j][s] = load16_any(x[j] + (kt * 128 + s * 32 + fq * 8) * 2);
+      }
+    }
+  }
+
+  // the row's last step: zeros past its end
+  __device__ __forceinline__ void load_end(const unsigned char* const (&w)[NF], const unsigned char* const (&ws)[NF],
+                                           const unsigned char* const (&x)[MT], const unsigned char* const (&xs)[MT], int kt, int fq, int blocks, int k) {
+    const int blk = kt * 4 + fq;
+    const bool live = blk < blocks;
+#pragma unroll
+    for (int i = 0; i < NF; ++i) {
+      wv[i] = make_uint4(0, 0, 0, 0);
+      if (live) wv[i] = *reinterpret_cast<const uint4*>(w[i] + blk * 16);
+      if constexpr (MX) wc[i] = live ? ws[i][blk] : 0;
+      else wc[i] = *reinterpret_cast<const unsigned*>(ws[i] + kt * 4);   // rows of scales are padded to four
+    }
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+      if constexpr (MX) {
+        xv[j][0] = make_uint4(0, 0, 0, 0);
+        xc[j] = 0;
+        if (live) {
+          xv[j][0] = *reinterpret_cast<const uint4*>(x[j] + blk * 16);
+          xc[j] = xs[j][blk];
+        }
+      } else {
+        const bf16_t* src = reinterpret_cast<const bf16_t*>(x[j]);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          const int col = kt * 128 + s * 32 + fq * 8, left = k - col;
+          xv[j][s] = make_uint4(0, 0, 0, 0);
+          if (left >= 8) {
+            xv[j][s] = load16_any(src + col);
+          } else if (left > 0) {
+            uint32_t h[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) h[e] = e < left ? src[col + e] : 0;
+            xv[j][s] = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+          }
+        }
+      }
+    }
+  }
+
+  __device__ __forceinline__ void multiply(f32x4_t (&acc)[NF][MT]) {
+#pragma unroll
+    for (int i = 0; i < NF; ++i) {
+      if constexpr (MX) {
+        const i32x8_t a = mx4_operand(wv[i]);
+#pragma unroll
+        for (int j = 0; j < MT; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, mx4_operand(xv[j][0]), acc[i][j], 4, 4, 0, (int)wc[i], 0, xc[j]);
+      } else {
+        turn_groups(wv[i]);
+        const unsigned q[4] = {wv[i].x, wv[i].y, wv[i].z, wv[i].w};
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          const float sc = __uint_as_float(((wc[i] >> (8 * s)) & 255u) << 23);
+          uint4 b;
+          b.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q[s], sc, 0));
+          b.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q[s], sc, 1));
+          b.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q[s], sc, 2));
+          b.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q[s], sc, 3));
+#pragma unroll
+          for (int j = 0; j < MT; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, b), __builtin_bit_cast(bf16x8_t, xv[j][s]), acc[i][j],
+                                                                0, 0, 0);
+        }
+      }
+    }
+  }
+};
+
+template <bool MX, int MT, int NF, typename OUT>
 __global__ void __launch_bounds__(512)
 mx4_rows_kernel(const Mx4Params p) {
   constexpr int NW = 8;
-  constexpr int U = MX ? 4 : (MT == 1 ? 4 : MT == 2 ? 2 : 1);   // steps whose loads are in flight
+  constexpr int U = MX ? 4 : (MT == 4 ? 1 : 2);            // steps whose loads are in flight
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   float4* const red = reinterpret_cast<float4*>(smem);     // [wave][NF * MT][64]
   const int tid = threadIdx.x, lane = tid & 63;
@@ -279,80 +452,39 @@ mx4_rows_kernel(const Mx4Params p) {
 #pragma unroll
     for (int j = 0; j < MT; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
-  for (int kt0 = wave; kt0 < p.nk; kt0 += NW * U) {
-    uint4 wv[U][NF], xv[U][MT][MX ? 1 : 4];
-    int wc[U][NF], xc[U][MT];
+  // rows past the ends read the last row's: their sums are never stored, and the loads need no branch
+  const unsigned char* wrow[NF];
+  const unsigned char* wsrow[NF];
+  const unsigned char* xrow[MT];
+  const unsigned char* xsrow[MT];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int blk = (kt0 + u * NW) * 4 + fq;
-      const bool live = blk < p.blocks;
+  for (int i = 0; i < NF; ++i) {
+    const long long n = min(n0 + i * 16 + fr, p.n - 1);
+    wrow[i] = p.w + n * rb;
+    wsrow[i] = p.ws + n * p.sstride;
+  }
 #pragma unroll
-      for (int i = 0; i < NF; ++i) {
-        const int n = n0 + i * 16 + fr;
-        wv[u][i] = make_uint4(0, 0, 0, 0);
-        wc[u][i] = 0;
-        if (live && n < p.n) {
-          wv[u][i] = *reinterpret_cast<const uint4*>(p.w + (long long)n * rb + blk * 16);
-          wc[u][i] = p.ws[(long long)n * p.sstride + blk];
-        }
-      }
+  for (int j = 0; j < MT; ++j) {
+    const long long m = min(m0 + j * 16 + fr, p.rows - 1);
+    xrow[j] = p.x + (MX ? m * rb : m * p.k * 2);
+    if constexpr (MX) xsrow[j] = p.xs + m * p.sstride;
+  }
+  RowsStep<MX, MT, NF> st[U];
+  const int full = MX ? p.blocks / 4 : p.k / 128;          // steps with every column there
+  constexpr int ROUND = NW * U;
+  const int rounds = full / ROUND;
+  int r = rounds > 0 ? (int)(blockIdx.x >> 3) % rounds : 0;
+  for (int i = 0; i < rounds; ++i) {
 #pragma unroll
-      for (int j = 0; j < MT; ++j) {
-        const long long m = m0 + j * 16 + fr;
-        const bool ok = live && m < p.rows;
-        xc[u][j] = 0;
-        if constexpr (MX) {
-          xv[u][j][0] = make_uint4(0, 0, 0, 0);
-          if (ok) {
-            xv[u][j][0] = *reinterpret_cast<const uint4*>(p.x + m * rb + blk * 16);
-            xc[u][j] = p.xs[m * p.sstride + blk];
-          }
-        } else {
-          const bf16_t* src = reinterpret_cast<const bf16_t*>(p.x) + m * p.k + blk * 32;
+    for (int u = 0; u < U; ++u) st[u].load(wrow, wsrow, xrow, xsrow, r * ROUND + u * NW + wave, fq);
 #pragma unroll
-          for (int s = 0; s < 4; ++s) {
-            xv[u][j][s] = make_uint4(0, 0, 0, 0);
-            const int left = p.k - (blk * 32 + 8 * s);
-            if (!ok || left <= 0) continue;
-            if (VEC) {                                     // k is a multiple of 8
-              xv[u][j][s] = *reinterpret_cast<const uint4*>(src + 8 * s);
-            } else {
-              uint32_t h[8];
-#pragma unroll
-              for (int e = 0; e < 8; ++e) h[e] = e < left ? src[8 * s + e] : 0;
-              xv[u][j][s] = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
-            }
-          }
-        }
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-#pragma unroll
-      for (int i = 0; i < NF; ++i) {
-        if constexpr (MX) {
-          const i32x8_t a = mx4_operand(wv[u][i]);
-#pragma unroll
-          for (int j = 0; j < MT; ++j)
-            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, mx4_operand(xv[u][j][0]), acc[i][j], 4, 4, 0, wc[u][i], 0, xc[u][j]);
-        } else {
-          const float sc = __uint_as_float((unsigned)wc[u][i] << 23);
-          const unsigned q[4] = {wv[u][i].x, wv[u][i].y, wv[u][i].z, wv[u][i].w};
-#pragma unroll
-          for (int s = 0; s < 4; ++s) {
-            uint4 b;
-            b.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q[s], sc, 0));
-            b.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q[s], sc, 1));
-            b.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q[s], sc, 2));
-            b.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q[s], sc, 3));
-#pragma unroll
-            for (int j = 0; j < MT; ++j)
-              acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, b), __builtin_bit_cast(bf16x8_t, xv[u][j][s]),
-                                                                  acc[i][j], 0, 0, 0);
-          }
-        }
-      }
-    }
+    for (int u = 0; u < U; ++u) st[u].multiply(acc);
+    r = r + 1 == rounds ? 0 : r + 1;
+  }
+  for (int kt = rounds * ROUND + wave; kt < p.nk; kt += NW) {
+    if (kt < full) st[0].load(wrow, wsrow, xrow, xsrow, kt, fq);
+    else st[0].load_end(wrow, wsrow, xrow, xsrow, kt, fq, p.blocks, p.k);
+    st[0].multiply(acc);
   }
 #pragma unroll
   for (int i = 0; i < NF; ++i)
@@ -396,43 +528,43 @@ static int mx_allow_lds(const char* what, K kern, int bytes, bool& done) {
   return LDM_OK;
 }
 
-template <int BM, int BN, int WM, int WN, int S, typename OUT>
+template <int BM, int BN, int WM, int WN, int S, bool MX, typename OUT>
 static int launch_mx4_gemm(Mx4Params& p, hipStream_t st) {
   p.tiles_m = (int)((p.rows + BM - 1) / BM);
   p.tiles_n = (p.n + BN - 1) / BN;
-  constexpr int smem = (BM + BN) * (S * 64 + 2 * 16);
-  auto kern = mx4_gemm_kernel<BM, BN, WM, WN, S, OUT>;
+  constexpr int smem = (BM + BN) * (S * 64 + (MX ? 2 * 16 : 0));
+  auto kern = mx4_gemm_kernel<BM, BN, WM, WN, S, MX, OUT>;
   static bool done = false;
   if (int rc = mx_allow_lds("ldm_mx4_linear", kern, smem, done)) return rc;
   hipLaunchKernelGGL(kern, dim3(p.tiles_m * p.tiles_n), dim3(64 * WM * WN), smem, st, p);
   return LDM_OK;
 }
 
-template <bool MX, int MT, int NF, bool VEC, typename OUT>
+template <bool MX, int MT, int NF, typename OUT>
 static int launch_mx4_rows(const Mx4Params& p, hipStream_t st) {
   constexpr int smem = 8 * NF * MT * 1024;
-  auto kern = mx4_rows_kernel<MX, MT, NF, VEC, OUT>;
+  auto kern = mx4_rows_kernel<MX, MT, NF, OUT>;
   static bool done = false;
   if (int rc = mx_allow_lds("ldm_mx4_linear", kern, smem, done)) return rc;
   hipLaunchKernelGGL(kern, dim3((p.n + 16 * NF - 1) / (16 * NF), (unsigned)((p.rows + 16 * MT - 1) / (16 * MT))), dim3(512), smem, st, p);
   return LDM_OK;
 }
 
-template <bool MX, bool VEC, typename OUT>
+template <bool MX, typename OUT>
 static int rows_by_size(const Mx4Params& p, hipStream_t st) {
   const bool wide = p.n >= 32 * 256;                       // two fragments of w a wave once every CU has a workgroup of them
-  if (p.rows <= 16) return wide ? launch_mx4_rows<MX, 1, 2, VEC, OUT>(p, st) : launch_mx4_rows<MX, 1, 1, VEC, OUT>(p, st);
-  if (p.rows <= 32) return launch_mx4_rows<MX, 2, 1, VEC, OUT>(p, st);
-  return launch_mx4_rows<MX, 4, 1, VEC, OUT>(p, st);
+  if (p.rows <= 16) return wide ? launch_mx4_rows<MX, 1, 2, OUT>(p, st) : launch_mx4_rows<MX, 1, 1, OUT>(p, st);
+  if (p.rows <= 32) return launch_mx4_rows<MX, 2, 1, OUT>(p, st);
+  return launch_mx4_rows<MX, 4, 1, OUT>(p, st);
 }
 
 template <typename OUT>
-static int mx4_linear_out(Mx4Params& p, bool mx, bool vec_x, hipStream_t st) {
-  if (!mx) return vec_x ? rows_by_size<false, true, OUT>(p, st) : rows_by_size<false, false, OUT>(p, st);
-  if (p.rows <= 64) return rows_by_size<true, true, OUT>(p, st);
+static int mx4_linear_out(Mx4Params& p, bool mx, hipStream_t st) {
+  if (!mx) return rows_by_size<false, OUT>(p, st);
+  if (p.rows <= 64) return rows_by_size<true, OUT>(p, st);
   const long long tiles = ((p.rows + 255) / 256) * ((p.n + 255) / 256);
-  if (tiles >= 128) return launch_mx4_gemm<256, 256, 2, 4, 4, OUT>(p, st);
-  return launch_mx4_gemm<128, 128, 2, 2, 4, OUT>(p, st);
+  if (tiles >= 128) return launch_mx4_gemm<256, 256, 2, 4, 4, true, OUT>(p, st);
+  return launch_mx4_gemm<128, 128, 2, 2, 4, true, OUT>(p, st);
 }
 
 }  // namespace ldm
@@ -461,8 +593,7 @@ extern "C" int ldm_mx4_linear(const void* x, const void* x_scale, const void* w,
   LDM_REQUIRE(rows <= 64LL * 65535 || mx, "ldm_mx4_linear: %lld rows of bfloat16", rows);
   LDM_REQUIRE(((rows + 127) / 128) * ((n + 127LL) / 128) < (1LL << 31), "ldm_mx4_linear: too large (rows=%lld n=%d)", rows, n);
   hipStream_t st = (hipStream_t)stream;
-  const bool vec_x = !mx && aligned16(x) && k % 8 == 0;
-  const int rc = out_dtype == LDM_BF16 ? mx4_linear_out<bf16_t>(p, mx, vec_x, st) : mx4_linear_out<float>(p, mx, vec_x, st);
+  const int rc = out_dtype == LDM_BF16 ? mx4_linear_out<bf16_t>(p, mx, st) : mx4_linear_out<float>(p, mx, st);
   if (rc) return rc;
   LDM_HIP_CHECK_LAUNCH("ldm_mx4_linear");
   return LDM_OK;

@@ -32,7 +32,6 @@ struct WgradMx8Params {
   int tiles_n, tiles_k;
   int steps_per_split, splits;
   int accumulate;              // direct form only
-  int vec_out;                 // 16-byte stores of `out` are legal
 };
 
 constexpr int WM8_MS = 64;     // rows a step: two MFMA contraction blocks
@@ -70,16 +69,16 @@ __device__ __attribute__((noinline)) void wm8_add(float* dst, int left, f32x4_t 
   for (int e = 0; e < 4; ++e)
     if (e < left) dst[e] += v[e];
 }
-__device__ __forceinline__ void wm8_store(float* dst, int left, f32x4_t v, int vec, int accumulate) {
+__device__ __forceinline__ void wm8_store(float* dst, int left, f32x4_t v, int accumulate) {
   if (left <= 0) return;
   if (accumulate) {
     wm8_add(dst, left, v);
-  } else if (vec) {                                        // k and the base are multiples of four floats: all four or none
-    *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (e < left) dst[e] = v[e];
+  } else if (left >= 4) {
+    store16_any(dst, make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])));
+  } else {                                                 // the end of a row
+    dst[0] = v[0];
+    if (left > 1) dst[1] = v[1];
+    if (left > 2) dst[2] = v[2];
   }
 }
 
@@ -340,7 +339,7 @@ linear_wgrad_mx8_kernel(const WgradMx8Params p) {
     float* row = out + (long long)n * p.k + k0 + w1 * (T1 / W1) + fq * 4;
     const int left = n < p.n ? p.k - (k0 + w1 * (T1 / W1) + fq * 4) : 0;
 #pragma unroll
-    for (int j = 0; j < F1; ++j) wm8_store(row + j * 16, left - j * 16, acc[i][j], p.vec_out, p.accumulate);
+    for (int j = 0; j < F1; ++j) wm8_store(row + j * 16, left - j * 16, acc[i][j], p.accumulate);
   }
 }
 
@@ -420,7 +419,6 @@ extern "C" int ldm_linear_wgrad_mx8(const void* x8, const void* x8_scale, const 
   p.rows = rows; p.n = n; p.k = k; p.blocks = mx_blocks(k); p.sstride = mx_scale_stride(k);
   p.out = need ? static_cast<float*>(workspace) : dw;
   p.accumulate = need ? 0 : accumulate;
-  p.vec_out = k % 4 == 0 && aligned16(p.out);
   hipStream_t st = (hipStream_t)stream;
   const int rc = cfg == 0   ? launch_wgrad_mx8<320, 160, 4, 2>(p, st)
                  : cfg == 1 ? launch_wgrad_mx8<256, 192, 4, 2>(p, st)
