@@ -39,8 +39,6 @@ __device__ __forceinline__ int mx_xcd_remap(int bid, int nblk) {
   return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (bid >> 3);
 }
 
-__device__ __forceinline__ i32x8_t mx4_operand(uint4 v) { return i32x8_t{(int)v.x, (int)v.y, (int)v.z, (int)v.w, 0, 0, 0, 0}; }
-
 // 16 / 4 bytes a lane from a raw buffer (base, bytes) into LDS, lane-linear from `lds`; a lane offset past `bytes` gives zeros
 __device__ __forceinline__ void mx_dma16(const void* base, unsigned bytes, unsigned char* lds, unsigned voff, int soff) {
   const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)bytes, 0x00020000);
@@ -321,107 +319,182 @@ mx4_gemm_kernel(const Mx4Params p) {
 }
 
 // --------------------------------------------------------------------------------------------------------- few rows
-// 16 NF rows of w and 16 MT rows of x a workgroup; its 8 waves take every 8th step of 128 columns and add up through LDS in a fixed
-// order.  Operands go straight from memory to registers (nothing is used twice by a wave), several steps' loads at once.
+// 16 NF rows of w and 16 MT rows of x a workgroup; its NW waves take a contiguous part of the columns each, 128 a step, and add up through
+// LDS in a fixed order.  What is to be had is the weights' bytes at the memory's rate, so every wave keeps S steps of its own in LDS
+// by LDS-DMA (no barrier: no wave reads another's), four or more consecutive lanes to a row.  Loading the matrix instructions'
+// fragments straight into registers -- consecutive lanes, different rows -- gives the address unit 16 bytes of every line at a
+// time: 31 us instead of 14 at 16 x 8192 x 10240 (42 MB of weights; 9 us at the rate of a large copy).
 //   MX  true: x in mx4, v_mfma_scale_f32_16x16x128_f8f6f4: lane l holds row l % 16, block l / 16 of the step
-//       false: x in bf16, four v_mfma_f32_16x16x32_bf16 a step, one for each block.  Lane group g = l / 16 of the s-th holds columns
-//              32 s + 8 g .. + 7 of x (a row's four lanes read 64 bytes in one piece: with the lane's own block, 32 g + 8 s, every load
-//              of x touched 64 pieces of 16 bytes).  The weights are loaded 16 bytes a lane -- block g -- and turned among the four
-//              groups: dword g of group s becomes dword s of group g, a 4 x 4 transposition in four lane-swap instructions.  They are
-//              widened to bf16 (exact: 2 significant bits) two at a time by the conversion that takes the scale along.
-typedef __attribute__((ext_vector_type(2))) unsigned int u32x2_t;
-__device__ __forceinline__ void turn_groups(uint4& v) {
-  u32x2_t a = __builtin_amdgcn_permlane32_swap(v.x, v.z, false, false), b = __builtin_amdgcn_permlane32_swap(v.y, v.w, false, false);
-  const u32x2_t c = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false), d = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
-  v = make_uint4(c[0], c[1], d[0], d[1]);
+//       false: x in bf16, four v_mfma_f32_16x16x32_bf16 a step.  Lane l holds row l % 16 again; the s-th takes columns 8 s .. + 7 of the
+//              lane's block l / 16, which are dword s of its weights, widened to bf16 (exact: 2 significant bits) two at a time by the
+//              conversion that takes the scale along, and chunk 4 (l / 16) + s of the 16 in the step's 256 bytes of x.
+// Chunks of a row are XOR-swizzled as in the tiles above: weights (64 bytes a row) by (row >> 1) & 3, x in bf16 (256) by row & 15.
+// DMAX: x can be fetched in 16-byte chunks (k a multiple of 8, x aligned); otherwise it goes through registers, zeros past the row's end.
+// until the LDS-DMA of all but the newest min(N, behind) steps of PER instructions has landed
+template <int N, int PER>
+__device__ __forceinline__ void wait_steps(int behind) {
+  if constexpr (N == 0) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  } else {
+    if (behind >= N) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N * PER) : "memory");
+    else wait_steps<N - 1, PER>(behind);
+  }
 }
 
-// a lane's operands of one step
-template <bool MX, int MT, int NF>
-struct RowsStep {
-  uint4 wv[NF], xv[MT][MX ? 1 : 4];
-  unsigned wc[NF];                                         // MX: the lane's scale byte; else the step's four
-  int xc[MT];
+template <bool MX, int MT, int NF, int NW, int S, bool DMAX, typename OUT>
+__global__ void __launch_bounds__(64 * NW)
+mx4_rows_kernel(const Mx4Params p) {
+  constexpr int XI = MX ? MT : 4 * MT;                     // x instructions of a step
+  constexpr int SLOT = (NF + XI) * 1024;
+  constexpr int SCALES = MX ? 2048 : 1024;                 // a group of four steps: 16 bytes a row
+  constexpr int WAVE = S * SLOT + 2 * SCALES;
+  constexpr int PER = NF + (DMAX ? XI : 0);                // LDS-DMA instructions of a step
+  constexpr unsigned OOB = 0x80000000u;
+  static_assert(NF * MT * 1024 <= WAVE && S <= 6 && (S - 1) * PER < 64, "LDS image");
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int fr = lane & 15, fq = lane >> 4;
+  const int n0 = blockIdx.x * (16 * NF);
+  const long long m0 = (long long)blockIdx.y * (16 * MT);
+  const int nk = p.nk, rb = p.blocks * 16, xb = MX ? rb : p.k * 2;
+  const int mrows = (int)min((long long)(16 * MT), p.rows - m0), nrows = min(16 * NF, p.n - n0);
+  const unsigned char* wbase = p.w + (long long)n0 * rb;
+  const unsigned char* wsbase = p.ws + (long long)n0 * p.sstride;
+  const unsigned char* xbase = p.x + m0 * xb;
+  const unsigned char* xsbase = MX ? p.xs + m0 * p.sstride : nullptr;
+  const unsigned wbytes = (unsigned)nrows * rb, xbytes = (unsigned)mrows * xb;
+  const unsigned wsbytes = (unsigned)nrows * p.sstride, xsbytes = (unsigned)mrows * p.sstride;
 
-  __device__ __forceinline__ void load(const unsigned char* const (&w)[NF], const unsigned char* const (&ws)[NF], const unsigned char* const (&x)[MT],
-                                       const unsigned char* const (&xs)[MT], int kt, int fq) {
-#pragma unroll
-    for (int i = 0; i < NF; ++i) {
-      wv[i] = *reinterpret_cast<const uint4*>(w[i] + kt * 64 + fq * 16);
-      if constexpr (MX) wc[i] = ws[i][kt * 4 + fq];
-      else wc[i] = *reinterpret_cast<const unsigned*>(ws[i] + kt * 4);
-    }
-#pragma unroll
-    for (int j = 0; j < MT; ++j) {
-      if constexpr (MX) {
-        xv[j][0] = *reinterpret_cast<const uint4*>(x[j] + kt * 64 + fq * 16);
-        xc[j] = xs[j][kt * 4 + fq];
+  const int per = (nk + NW - 1) / NW, s0 = wave * per, s1 = min(s0 + per, nk);
+  const bool word_scales = nk < 4;                         // rows of less than 16 bytes of scales: a step at a time
+  unsigned char* const mine = smem + wave * WAVE;
+  const int wchunk = (lane & 3) ^ ((lane >> 3) & 3);
+  const unsigned wvoff = (unsigned)(lane >> 2) * rb + wchunk * 16;
+  const int srow = 16 * NF;
+
+  auto stage = [&](int kt) {
+    if (((kt - s0) & 3) == 0) {
+      unsigned char* dst = mine + S * SLOT + (((kt - s0) >> 2) & 1) * SCALES;
+      const unsigned wo = lane < srow ? (unsigned)lane * p.sstride : OOB, xo = lane < 16 * MT ? (unsigned)lane * p.sstride : OOB;
+      if (word_scales) {
+        mx_dma4(wsbase, wsbytes, dst, wo, kt * 4);
+        if constexpr (MX) mx_dma4(xsbase, xsbytes, dst + 1024, xo, kt * 4);
       } else {
-#pragma unroll
-        for (int s = 0; s < 4; ++s) xv[j][s] = load16_any(x[j] + (kt * 128 + s * 32 + fq * 8) * 2);
+        const int first = min(kt, nk - 4) * 4;             // the last fetch ends with the row
+        mx_dma16(wsbase, wsbytes, dst, wo, first);
+        if constexpr (MX) mx_dma16(xsbase, xsbytes, dst + 1024, xo, first);
       }
     }
-  }
-
-  // the row's last step: zeros past its end
-  __device__ __forceinline__ void load_end(const unsigned char* const (&w)[NF], const unsigned char* const (&ws)[NF],
-                                           const unsigned char* const (&x)[MT], const unsigned char* const (&xs)[MT], int kt, int fq, int blocks, int k) {
-    const int blk = kt * 4 + fq;
-    const bool live = blk < blocks;
+    unsigned char* dst = mine + (kt - s0) % S * SLOT;
+    const bool past = kt * 4 + wchunk >= p.blocks;
 #pragma unroll
-    for (int i = 0; i < NF; ++i) {
-      wv[i] = make_uint4(0, 0, 0, 0);
-      if (live) wv[i] = *reinterpret_cast<const uint4*>(w[i] + blk * 16);
-      if constexpr (MX) wc[i] = live ? ws[i][blk] : 0;
-      else wc[i] = *reinterpret_cast<const unsigned*>(ws[i] + kt * 4);   // rows of scales are padded to four
-    }
+    for (int i = 0; i < NF; ++i) mx_dma16(wbase, wbytes, dst + i * 1024, past ? OOB : wvoff + i * 16 * rb, kt * 64);
+    dst += NF * 1024;
+    if constexpr (MX) {
 #pragma unroll
-    for (int j = 0; j < MT; ++j) {
-      if constexpr (MX) {
-        xv[j][0] = make_uint4(0, 0, 0, 0);
-        xc[j] = 0;
-        if (live) {
-          xv[j][0] = *reinterpret_cast<const uint4*>(x[j] + blk * 16);
-          xc[j] = xs[j][blk];
-        }
-      } else {
-        const bf16_t* src = reinterpret_cast<const bf16_t*>(x[j]);
+      for (int j = 0; j < MT; ++j) mx_dma16(xbase, xbytes, dst + j * 1024, past ? OOB : wvoff + j * 16 * rb, kt * 64);
+    } else {
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          const int col = kt * 128 + s * 32 + fq * 8, left = k - col;
-          xv[j][s] = make_uint4(0, 0, 0, 0);
+      for (int t = 0; t < XI; ++t) {
+        const int row = 4 * t + fq, chunk = fr ^ (row & 15), col = kt * 128 + chunk * 8;
+        if constexpr (DMAX) {
+          mx_dma16(xbase, xbytes, dst + t * 1024, col >= p.k ? OOB : (unsigned)row * xb + chunk * 16, kt * 256);
+        } else {
+          uint4 v = make_uint4(0, 0, 0, 0);
+          const int left = row >= mrows ? 0 : p.k - col;
+          const bf16_t* src = reinterpret_cast<const bf16_t*>(xbase + (long long)row * xb) + col;
           if (left >= 8) {
-            xv[j][s] = load16_any(src + col);
+            v = load16_any(src);
           } else if (left > 0) {
             uint32_t h[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) h[e] = e < left ? src[col + e] : 0;
-            xv[j][s] = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+            for (int e = 0; e < 8; ++e) h[e] = e < left ? src[e] : 0;
+            v = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
           }
+          *reinterpret_cast<uint4*>(dst + t * 1024 + lane * 16) = v;
         }
       }
     }
-  }
+  };
 
-  __device__ __forceinline__ void multiply(f32x4_t (&acc)[NF][MT]) {
+  f32x4_t acc[NF][MT];
+#pragma unroll
+  for (int i = 0; i < NF; ++i)
+#pragma unroll
+    for (int j = 0; j < MT; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+
+  const unsigned lds = (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)mine;
+  const unsigned waddr = lds + fr * 64 + ((fq ^ ((fr >> 1) & 3)) << 4);
+  unsigned xaddr[4];
+#pragma unroll
+  for (int s = 0; s < 4; ++s) xaddr[s] = lds + NF * 1024 + fr * 256 + (((4 * fq + s) ^ fr) << 4);
+  const int sstep = word_scales ? 4 : 16;
+  const unsigned saddr = lds + S * SLOT + fr * sstep;
+
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s)
+    if (s0 + s < s1) stage(s0 + s);
+  for (int kt = s0; kt < s1; ++kt) {
+    if (kt + S - 1 < s1) stage(kt + S - 1);                // into the slot of the step before this one
+    wait_steps<S - 1, PER>(s1 - 1 - kt);
+    LDM_LOCKSTEP();
+    const unsigned slot = (unsigned)((kt - s0) % S) * SLOT;
+    const int g = (kt - s0) >> 2, word = word_scales ? 0 : kt - min(s0 + 4 * g, nk - 4);
+    const unsigned sa = saddr + (g & 1) * SCALES + word * 4;
+    i32x4_t wv[NF], xv[MT][MX ? 1 : 4];
+    int wc[NF], xc[MT];
+#pragma unroll
+    for (int i = 0; i < NF; ++i) lds_read4<0>(wc[i], sa + i * 16 * sstep);
+    if constexpr (MX) {
+#pragma unroll
+      for (int j = 0; j < MT; ++j) lds_read4<1024>(xc[j], sa + j * 16 * sstep);
+    }
+    [&]<int... I>(std::integer_sequence<int, I...>) {
+      (lds_read16<I * 1024>(wv[I], waddr + slot), ...);
+    }(std::make_integer_sequence<int, NF>{});
+    [&]<int... J>(std::integer_sequence<int, J...>) {
+      ([&] {
+        constexpr int j = J;
+        if constexpr (MX) {
+          lds_read16<(NF + j) * 1024>(xv[j][0], waddr + slot);
+        } else {
+          lds_read16<j * 4096>(xv[j][0], xaddr[0] + slot);
+          lds_read16<j * 4096>(xv[j][1], xaddr[1] + slot);
+          lds_read16<j * 4096>(xv[j][2], xaddr[2] + slot);
+          lds_read16<j * 4096>(xv[j][3], xaddr[3] + slot);
+        }
+      }(), ...);
+    }(std::make_integer_sequence<int, MT>{});
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < NF; ++i) asm volatile("" : "+v"(wv[i]), "+v"(wc[i]));   // no use moves above the wait
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+      if constexpr (MX) asm volatile("" : "+v"(xc[j]));
+#pragma unroll
+      for (int s = 0; s < (MX ? 1 : 4); ++s) asm volatile("" : "+v"(xv[j][s]));
+    }
 #pragma unroll
     for (int i = 0; i < NF; ++i) {
+      const unsigned code = ((unsigned)wc[i] >> (8 * fq)) & 255u;
       if constexpr (MX) {
-        const i32x8_t a = mx4_operand(wv[i]);
+        const i32x8_t a{wv[i][0], wv[i][1], wv[i][2], wv[i][3], 0, 0, 0, 0};
 #pragma unroll
-        for (int j = 0; j < MT; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, mx4_operand(xv[j][0]), acc[i][j], 4, 4, 0, (int)wc[i], 0, xc[j]);
+        for (int j = 0; j < MT; ++j) {
+          const i32x8_t b{xv[j][0][0], xv[j][0][1], xv[j][0][2], xv[j][0][3], 0, 0, 0, 0};
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc[i][j], 4, 4, 0, (int)code, 0, (int)((unsigned)xc[j] >> (8 * fq)));
+        }
       } else {
-        turn_groups(wv[i]);
-        const unsigned q[4] = {wv[i].x, wv[i].y, wv[i].z, wv[i].w};
+        const float sc = __uint_as_float(code << 23);
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-          const float sc = __uint_as_float(((wc[i] >> (8 * s)) & 255u) << 23);
+          const unsigned q = (unsigned)wv[i][s];
           uint4 b;
-          b.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q[s], sc, 0));
-          b.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q[s], sc, 1));
-          b.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q[s], sc, 2));
-          b.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q[s], sc, 3));
+          b.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, sc, 0));
+          b.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, sc, 1));
+          b.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, sc, 2));
+          b.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, sc, 3));
 #pragma unroll
           for (int j = 0; j < MT; ++j)
             acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, b), __builtin_bit_cast(bf16x8_t, xv[j][s]), acc[i][j],
@@ -430,77 +503,23 @@ struct RowsStep {
       }
     }
   }
-};
-
-template <bool MX, int MT, int NF, typename OUT>
-__global__ void __launch_bounds__(512)
-mx4_rows_kernel(const Mx4Params p) {
-  constexpr int NW = 8;
-  constexpr int U = MX ? 4 : (MT == 4 ? 1 : 2);            // steps whose loads are in flight
-  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  float4* const red = reinterpret_cast<float4*>(smem);     // [wave][NF * MT][64]
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int fr = lane & 15, fq = lane >> 4;
-  const int n0 = blockIdx.x * (16 * NF);
-  const long long m0 = (long long)blockIdx.y * (16 * MT);
-  const int rb = p.blocks * 16;
-
-  f32x4_t acc[NF][MT];
-#pragma unroll
-  for (int i = 0; i < NF; ++i)
-#pragma unroll
-    for (int j = 0; j < MT; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-
-  // rows past the ends read the last row's: their sums are never stored, and the loads need no branch
-  const unsigned char* wrow[NF];
-  const unsigned char* wsrow[NF];
-  const unsigned char* xrow[MT];
-  const unsigned char* xsrow[MT];
-#pragma unroll
-  for (int i = 0; i < NF; ++i) {
-    const long long n = min(n0 + i * 16 + fr, p.n - 1);
-    wrow[i] = p.w + n * rb;
-    wsrow[i] = p.ws + n * p.sstride;
-  }
-#pragma unroll
-  for (int j = 0; j < MT; ++j) {
-    const long long m = min(m0 + j * 16 + fr, p.rows - 1);
-    xrow[j] = p.x + (MX ? m * rb : m * p.k * 2);
-    if constexpr (MX) xsrow[j] = p.xs + m * p.sstride;
-  }
-  RowsStep<MX, MT, NF> st[U];
-  const int full = MX ? p.blocks / 4 : p.k / 128;          // steps with every column there
-  constexpr int ROUND = NW * U;
-  const int rounds = full / ROUND;
-  int r = rounds > 0 ? (int)(blockIdx.x >> 3) % rounds : 0;
-  for (int i = 0; i < rounds; ++i) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) st[u].load(wrow, wsrow, xrow, xsrow, r * ROUND + u * NW + wave, fq);
-#pragma unroll
-    for (int u = 0; u < U; ++u) st[u].multiply(acc);
-    r = r + 1 == rounds ? 0 : r + 1;
-  }
-  for (int kt = rounds * ROUND + wave; kt < p.nk; kt += NW) {
-    if (kt < full) st[0].load(wrow, wsrow, xrow, xsrow, kt, fq);
-    else st[0].load_end(wrow, wsrow, xrow, xsrow, kt, fq, p.blocks, p.k);
-    st[0].multiply(acc);
-  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  LDM_LOCKSTEP();
 #pragma unroll
   for (int i = 0; i < NF; ++i)
 #pragma unroll
     for (int j = 0; j < MT; ++j)
-      red[(wave * NF * MT + i * MT + j) * 64 + lane] = make_float4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
+      reinterpret_cast<float4*>(mine)[(i * MT + j) * 64 + lane] = make_float4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
   __syncthreads();
-  for (int t = tid; t < NF * MT * 64; t += 512) {
+  for (int t = tid; t < NF * MT * 64; t += 64 * NW) {
     const int f = t >> 6, l = t & 63, i = f / MT, j = f - i * MT;
     const int n = n0 + i * 16 + (l >> 4) * 4;
     const long long m = m0 + j * 16 + (l & 15);
     if (m >= p.rows || n >= p.n) continue;
-    float4 s = red[t];
+    float4 s = reinterpret_cast<const float4*>(smem)[t];
 #pragma unroll
     for (int w = 1; w < NW; ++w) {
-      const float4 o = red[w * NF * MT * 64 + t];
+      const float4 o = reinterpret_cast<const float4*>(smem + w * WAVE)[t];
       s.x += o.x; s.y += o.y; s.z += o.z; s.w += o.w;
     }
     float v[4] = {s.x, s.y, s.z, s.w};
@@ -540,28 +559,40 @@ static int launch_mx4_gemm(Mx4Params& p, hipStream_t st) {
   return LDM_OK;
 }
 
-template <bool MX, int MT, int NF, typename OUT>
+template <bool MX, int MT, int NF, int NW, int S, bool DMAX, typename OUT>
 static int launch_mx4_rows(const Mx4Params& p, hipStream_t st) {
-  constexpr int smem = 8 * NF * MT * 1024;
-  auto kern = mx4_rows_kernel<MX, MT, NF, OUT>;
+  constexpr int smem = NW * (S * (NF + (MX ? MT : 4 * MT)) * 1024 + (MX ? 4096 : 2048));
+  auto kern = mx4_rows_kernel<MX, MT, NF, NW, S, DMAX, OUT>;
   static bool done = false;
   if (int rc = mx_allow_lds("ldm_mx4_linear", kern, smem, done)) return rc;
-  hipLaunchKernelGGL(kern, dim3((p.n + 16 * NF - 1) / (16 * NF), (unsigned)((p.rows + 16 * MT - 1) / (16 * MT))), dim3(512), smem, st, p);
+  hipLaunchKernelGGL(kern, dim3((p.n + 16 * NF - 1) / (16 * NF), (unsigned)((p.rows + 16 * MT - 1) / (16 * MT))), dim3(64 * NW), smem, st, p);
   return LDM_OK;
 }
 
-template <bool MX, typename OUT>
+template <bool MX, bool DMAX, typename OUT>
 static int rows_by_size(const Mx4Params& p, hipStream_t st) {
-  const bool wide = p.n >= 32 * 256;                       // two fragments of w a wave once every CU has a workgroup of them
-  if (p.rows <= 16) return wide ? launch_mx4_rows<MX, 1, 2, OUT>(p, st) : launch_mx4_rows<MX, 1, 1, OUT>(p, st);
-  if (p.rows <= 32) return launch_mx4_rows<MX, 2, 1, OUT>(p, st);
-  return launch_mx4_rows<MX, 4, 1, OUT>(p, st);
+  // Fragments of w a workgroup: as many as leave every CU one workgroup of its own (n = 8192 / 10240, 16 rows, k = 8192: 12.4 / 14.3 us;
+  // with two fragments throughout 12.4 / 19.2, since some CUs then have two workgroups and some one).  Waves and steps: what LDS holds.
+  const int nf = (p.n + 4095) / 4096;
+  if (p.rows <= 16) {
+    if (nf == 1) return launch_mx4_rows<MX, 1, 1, 8, 2, DMAX, OUT>(p, st);
+    if (nf == 2) return launch_mx4_rows<MX, 1, 2, 8, 3, DMAX, OUT>(p, st);
+    if (nf == 3) return launch_mx4_rows<MX, 1, 3, 8, 2, DMAX, OUT>(p, st);
+    if (nf == 4) return launch_mx4_rows<MX, 1, 4, 8, 2, DMAX, OUT>(p, st);
+    return launch_mx4_rows<MX, 1, 2, 4, 3, DMAX, OUT>(p, st);   // several rounds of workgroups: two a CU at a time
+  }
+  if (p.rows <= 32) {
+    if (nf == 1) return launch_mx4_rows<MX, 2, 1, 8, 2, DMAX, OUT>(p, st);
+    return launch_mx4_rows<MX, 2, 2, 4, 3, DMAX, OUT>(p, st);
+  }
+  if (nf == 1) return launch_mx4_rows<MX, 4, 1, MX ? 8 : 4, MX ? 3 : 2, DMAX, OUT>(p, st);
+  return launch_mx4_rows<MX, 4, 2, 4, MX ? 4 : 2, DMAX, OUT>(p, st);
 }
 
 template <typename OUT>
 static int mx4_linear_out(Mx4Params& p, bool mx, hipStream_t st) {
-  if (!mx) return rows_by_size<false, OUT>(p, st);
-  if (p.rows <= 64) return rows_by_size<true, OUT>(p, st);
+  if (!mx) return p.k % 8 == 0 && aligned16(p.x) ? rows_by_size<false, true, OUT>(p, st) : rows_by_size<false, false, OUT>(p, st);
+  if (p.rows <= 64) return rows_by_size<true, true, OUT>(p, st);
   const long long tiles = ((p.rows + 255) / 256) * ((p.n + 255) / 256);
   if (tiles >= 128) return launch_mx4_gemm<256, 256, 2, 4, 4, true, OUT>(p, st);
   return launch_mx4_gemm<128, 128, 2, 2, 4, true, OUT>(p, st);
