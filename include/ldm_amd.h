@@ -452,6 +452,10 @@ int ldm_glu_backward_mx8(const void* data, const void* scale, const void* dout, 
 int ldm_mx4_linear(const void* x, const void* x_scale, const void* w, const void* w_scale, const float* bias, void* out, int out_dtype,
                    long long rows, int n, int k, void* stream);
 
+/* out (rows, n) = x W^T + bias for plain bfloat16 operands x (rows, k), w (n, k), contiguous, 16-byte aligned, k a multiple of 8 up to
+ * 2^21: the product behind ldm_mx_dequantize / ldm_mx4_dequantize_t, for many rows.  bias, out, sums as above. */
+int ldm_linear_bf16(const void* x, const void* w, const float* bias, void* out, int out_dtype, long long rows, int n, int k, void* stream);
+
 /* dw (n, k) float32 (+)= dY^T X: weight gradient of a linear layer whose input was kept in LDM_MX8.  dy (rows, n) bfloat16, contiguous,
  * 16-byte aligned, n a multiple of 8; x8 / x8_scale (rows, k).  Sums are float32 in a fixed order (no atomics).  `workspace` of
  * ldm_linear_wgrad_mx8_workspace_bytes (may be 0: NULL is fine then), 16-byte aligned. */

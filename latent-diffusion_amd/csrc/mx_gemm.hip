@@ -59,6 +59,9 @@ template <int OFF>
 __device__ __forceinline__ void lds_read4(int& v, unsigned addr) {
   asm volatile("ds_read_b32 %0, %1 offset:%2" : "=v"(v) : "v"(addr), "n"(OFF) : "memory");
 }
+// no use of v moves above the wait in front of this
+__device__ __forceinline__ void stay_below(i32x4_t& v) { asm volatile("" : "+v"(v)); }
+
 template <bool MX, int H>
 __device__ __forceinline__ void mx_mfma(f32x16_t& c, i32x4_t a, i32x4_t b, int sa, int sb) {
   if constexpr (MX)
@@ -66,6 +69,68 @@ __device__ __forceinline__ void mx_mfma(f32x16_t& c, i32x4_t a, i32x4_t b, int s
                                                         2 * H, sa, 2 * H, sb);
   else
     c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+}
+
+// A wave's MI x NI tiles of 32 x 32 (register r of tile (i, j): column n0 + 32 j + 8 (r / 4) + 4 (lane / 32) + r % 4, row m0 + 32 i + lane % 32)
+// plus bias into the output: 32 rows at a time through the wave's own LDS, then whole 16-byte pieces of rows.
+template <int NI, typename OUT>
+constexpr int store_pitch() { return NI * 32 * (int)sizeof(OUT) + 16; }
+template <int MI, int NI, typename OUT>
+__device__ __forceinline__ void store_tiles(const Mx4Params& p, const f32x16_t (&acc)[MI][NI], unsigned char* cst, long long m0, int n0, int lane) {
+  constexpr int WTN = NI * 32;
+  const int fr = lane & 31, fh = lane >> 5;
+  constexpr int PITCH = store_pitch<NI, OUT>();
+  constexpr int EPR = 16 / (int)sizeof(OUT);               // elements of a piece
+  float bv[NI][4][4];
+  if (p.bias != nullptr) {
+#pragma unroll
+    for (int j = 0; j < NI; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) bv[j][q][e] = p.bias[min(n0 + j * 32 + 8 * q + 4 * fh + e, p.n - 1)];
+  } else {
+#pragma unroll
+    for (int j = 0; j < NI; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) bv[j][q][e] = 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+#pragma unroll
+    for (int j = 0; j < NI; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * q + e] + bv[j][q][e];
+        unsigned char* d = cst + fr * PITCH + (j * 32 + 8 * q + 4 * fh) * (int)sizeof(OUT);
+        if constexpr (sizeof(OUT) == 2) *reinterpret_cast<uint2*>(d) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+        else *reinterpret_cast<float4*>(d) = make_float4(v[0], v[1], v[2], v[3]);
+      }
+    LDM_LOCKSTEP();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    constexpr int PPR = WTN / EPR;                         // pieces a row
+#pragma unroll 4
+    for (int t = 0; t < 32 * PPR / 64; ++t) {
+      const int piece = t * 64 + lane, r = piece / PPR, c = (piece - r * PPR) * EPR;
+      const long long m = m0 + i * 32 + r;
+      const int n = n0 + c;
+      if (m >= p.rows || n >= p.n) continue;
+      OUT* dst = static_cast<OUT*>(p.out) + m * p.n + n;
+      const unsigned char* s = cst + r * PITCH + c * (int)sizeof(OUT);
+      if (n + EPR <= p.n) {
+        store16_any(dst, *reinterpret_cast<const uint4*>(s));
+      } else {                                             // the end of a row
+#pragma unroll 1
+        for (int e = 0; n + e < p.n; ++e) dst[e] = reinterpret_cast<const OUT*>(s)[e];
+      }
+    }
+    LDM_LOCKSTEP();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
 }
 
 // Tile of BM (rows of x) x BN (rows of w) by WM x WN waves; a step is 64 bytes of every row (MX: 128 columns of mx4, four blocks; else 32
@@ -261,60 +326,165 @@ mx4_gemm_kernel(const Mx4Params p) {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();                                         // the slots become the epilogue's
 
-  // ---- epilogue: 32 rows of the wave's tile at a time through its own LDS, then whole 16-byte pieces of rows
-  constexpr int PITCH = WTN * (int)sizeof(OUT) + 16;
-  constexpr int EPR = 16 / (int)sizeof(OUT);               // elements of a piece
-  static_assert(WM * WN * 32 * PITCH <= S * STAGE + 2 * SCALES, "epilogue image");
-  unsigned char* const cst = smem + wave * 32 * PITCH;
-  float bv[NI][4][4];
-  if (p.bias != nullptr) {
+  static_assert(WM * WN * 32 * store_pitch<NI, OUT>() <= S * STAGE + 2 * SCALES, "epilogue image");
+  store_tiles<MI, NI, OUT>(p, acc, smem + wave * 32 * store_pitch<NI, OUT>(), m0 + wm * WTM, n0 + wn * WTN, lane);
+}
+
+// ------------------------------------------------------------------------------------------------- plain bf16 operands
+// out = x W^T + bias for bf16 rows: the product behind the widening of the weights.  A step is 64 columns (128 bytes) of every row: the
+// chip's L2 hands out lines of 128 bytes, and LDS-DMA of 64 of them a row gets half the rate (17 against 29 TB/s over all CUs).  Chunks
+// are swizzled by row & 7.  The registers of a whole step -- four rounds of v_mfma_f32_32x32x16_bf16 -- are read while the step before
+// multiplies, one barrier a step.  What bounds the loop is LDS: a wave's tile of 64 x 64 reads as many bytes as its instructions take
+// time, 32 x 160 and 64 x 160 fewer.
+//   KW == 1: WM x WN waves share a tile of BM x BN.
+//   KW > 1:  few tiles, where a launch is as long as one workgroup's chain of steps: the KW waves of a workgroup each take a contiguous part
+//            of the columns of the whole tile, with a ring of their own and no barrier, and add up through LDS in a fixed order.
+// Steps past the end are fetched as zeros, so the number of steps is rounded up to an even one.
+template <int BM, int BN, int WM, int WN, int KW, int S, typename OUT>
+__global__ void __launch_bounds__(64 * WM * WN * KW, KW > 1 || BM * BN > 16384 ? 1 : 2)
+bf16_gemm_kernel(const Mx4Params p) {
+  static_assert(KW == 1 || (WM == 1 && WN == 1), "a wave of its own tile or of its own columns");
+  constexpr int NT = 64 * WM * WN, ROWS = BM + BN;
+  constexpr int IT = ROWS * 8 / NT;                        // DMA instructions of a wave a step
+  constexpr int STAGE = ROWS * 128, RING = S * STAGE;
+  constexpr int WTM = BM / WM, WTN = BN / WN, MI = WTM / 32, NI = WTN / 32;
+  constexpr unsigned OOB = 0x80000000u;
+  static_assert(BM * 8 % NT == 0 && BN * 8 % NT == 0 && (S - 2) * IT < 64, "tile / threads mismatch");
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kw = KW > 1 ? wave : 0, gw = KW > 1 ? 0 : wave;
+  const int gt = KW > 1 ? lane : tid;                      // thread of the group that shares a ring
+  const int wm = gw / WN, wn = gw % WN;
+  const int fr = lane & 31, fh = lane >> 5;
+
+  const int tile = mx_xcd_remap(blockIdx.x, gridDim.x);
+  const int band = 4 * p.tiles_n, g4 = tile / band, in = tile - g4 * band;
+  const int brows = min(p.tiles_m - g4 * 4, 4);
+  const int tn = in / brows, tm = g4 * 4 + (in - tn * brows);
+  const long long m0 = (long long)tm * BM;
+  const int n0 = tn * BN;
+
+  const int rb = p.k * 2, chunks = p.k >> 3;
+  const unsigned char* xbase = p.x + m0 * rb;
+  const unsigned char* wbase = p.w + (long long)n0 * rb;
+  const unsigned xbytes = (unsigned)min((long long)BM, p.rows - m0) * rb, wbytes = (unsigned)min(BN, p.n - n0) * rb;
+  const int chunk = (gt & 7) ^ ((gt >> 3) & 7);
+  const unsigned voff = (unsigned)(gt >> 3) * rb + chunk * 16;
+
+  const int per = ((p.nk + KW - 1) / KW + 1) & ~1, s0 = kw * per;
+  unsigned char* const ring = smem + kw * RING;
+  auto stage_part = [&](int kt, int it) {                  // instruction `it` of step s0 + kt
+    unsigned char* dst = ring + (kt % S) * STAGE + gw * 1024 + it * NT * 16;
+    const bool past = kt >= per || (s0 + kt) * 8 + chunk >= chunks;
+    const int so = (s0 + kt) * 128;
+    if (it * NT < BM * 8) mx_dma16(xbase, xbytes, dst, past ? OOB : voff + it * (NT / 8) * rb, so);
+    else mx_dma16(wbase, wbytes, dst, past ? OOB : voff + (it * (NT / 8) - BM) * rb, so);
+  };
+  auto stage = [&](int kt) {
+#pragma unroll
+    for (int it = 0; it < IT; ++it) stage_part(kt, it);
+  };
+
+  f32x16_t acc[MI][NI];
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
 #pragma unroll
     for (int j = 0; j < NI; ++j)
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) bv[j][q][e] = p.bias[min(n0 + wn * WTN + j * 32 + 8 * q + 4 * fh + e, p.n - 1)];
-  } else {
-#pragma unroll
-    for (int j = 0; j < NI; ++j)
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) bv[j][q][e] = 0.f;
-  }
-#pragma unroll
-  for (int i = 0; i < MI; ++i) {
-#pragma unroll
-    for (int j = 0; j < NI; ++j)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        float v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * q + e] + bv[j][q][e];
-        unsigned char* d = cst + fr * PITCH + (j * 32 + 8 * q + 4 * fh) * (int)sizeof(OUT);
-        if constexpr (sizeof(OUT) == 2) *reinterpret_cast<uint2*>(d) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
-        else *reinterpret_cast<float4*>(d) = make_float4(v[0], v[1], v[2], v[3]);
-      }
-    LDM_LOCKSTEP();
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+
+  i32x4_t xf[2][4][MI], wf[2][4][NI];                      // [set][round of the step]
+  const unsigned lds = (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)ring;
+  const int swz = fr & 7;
+  const unsigned xaddr = lds + (wm * WTM + fr) * 128 + ((fh ^ swz) << 4), waddr = lds + (BM + wn * WTN + fr) * 128 + ((fh ^ swz) << 4);
+  constexpr int READS = 4 * (MI + NI), MM = 4 * MI * NI;
+  auto read = [&]<int SET, int Q>(std::integral_constant<int, SET>, std::integral_constant<int, Q>, unsigned slot) {
+    constexpr int h = Q / (MI + NI), q = Q % (MI + NI), i = q < MI ? q : 0, j = q < MI ? 0 : q - MI;
+    if constexpr (q < MI) lds_read16<i * 4096>(xf[SET][h][i], (xaddr ^ (h * 32)) + slot);
+    else lds_read16<j * 4096>(wf[SET][h][j], (waddr ^ (h * 32)) + slot);
+  };
+  auto landed = [&]<int SET>(std::integral_constant<int, SET>) {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    constexpr int PPR = WTN / EPR;                         // pieces a row
-#pragma unroll 4
-    for (int t = 0; t < 32 * PPR / 64; ++t) {
-      const int piece = t * 64 + lane, r = piece / PPR, c = (piece - r * PPR) * EPR;
-      const long long m = m0 + wm * WTM + i * 32 + r;
-      const int n = n0 + wn * WTN + c;
-      if (m >= p.rows || n >= p.n) continue;
-      OUT* dst = static_cast<OUT*>(p.out) + m * p.n + n;
-      const unsigned char* s = cst + r * PITCH + c * (int)sizeof(OUT);
-      if (n + EPR <= p.n) {
-        store16_any(dst, *reinterpret_cast<const uint4*>(s));
-      } else {                                             // the end of a row
-#pragma unroll 1
-        for (int e = 0; n + e < p.n; ++e) dst[e] = reinterpret_cast<const OUT*>(s)[e];
-      }
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+#pragma unroll
+      for (int i = 0; i < MI; ++i) stay_below(xf[SET][h][i]);
+#pragma unroll
+      for (int j = 0; j < NI; ++j) stay_below(wf[SET][h][j]);
     }
+  };
+  auto next_here = [&] {                                   // the next step's DMA has landed, and the slot of this one is free
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 2) * IT) : "memory");
+    if constexpr (KW == 1) __builtin_amdgcn_s_barrier();
+    else LDM_LOCKSTEP();
+    asm volatile("" ::: "memory");
+  };
+  // step kt from register set SET; the next one's reads between the matrix instructions
+  auto step = [&]<int SET>(std::integral_constant<int, SET>, int kt) {
+    next_here();
+    const unsigned slot = (unsigned)((kt + 1) % S) * STAGE;
+    [&]<int... Q>(std::integer_sequence<int, Q...>) {
+      ([&] {
+        constexpr int q = Q, h = q / (MI * NI), i = q / NI % MI, j = q % NI;
+        mx_mfma<false, h>(acc[i][j], wf[SET][h][j], xf[SET][h][i], 0, 0);
+        // two reads at a time: all are out by the middle of the step
+        if constexpr (2 * q < READS) read(std::integral_constant<int, 1 - SET>{}, std::integral_constant<int, 2 * q>{}, slot);
+        if constexpr (2 * q + 1 < READS) read(std::integral_constant<int, 1 - SET>{}, std::integral_constant<int, 2 * q + 1>{}, slot);
+        // the DMA spread likewise: issued in one go it holds the wave up for as long as it takes
+#pragma unroll
+        for (int it = q * IT / MM; it < (q + 1) * IT / MM; ++it) stage_part(kt + S, it);
+        __builtin_amdgcn_sched_barrier(0);
+      }(), ...);
+    }(std::make_integer_sequence<int, MM>{});
+    landed(std::integral_constant<int, 1 - SET>{});
+  };
+  constexpr std::integral_constant<int, 0> SET0{};
+  constexpr std::integral_constant<int, 1> SET1{};
+  static_assert(READS <= 2 * MM, "every read has its place");
+
+#pragma unroll
+  for (int t = 0; t < S - 1; ++t) stage(t);
+  next_here();
+  stage(S - 1);
+  [&]<int... Q>(std::integer_sequence<int, Q...>) {
+    (read(SET0, std::integral_constant<int, Q>{}, 0u), ...);
+  }(std::make_integer_sequence<int, READS>{});
+  landed(SET0);
+  for (int kt = 0; kt < per; kt += 2) {
+    step(SET0, kt);
+    step(SET1, kt + 1);
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  if constexpr (KW == 1) {
+    __syncthreads();                                       // the slots become the epilogue's
+    static_assert(KW > 1 || WM * WN * 32 * store_pitch<NI, OUT>() <= RING, "epilogue image");
+    store_tiles<MI, NI, OUT>(p, acc, smem + wave * 32 * store_pitch<NI, OUT>(), m0 + wm * WTM, n0 + wn * WTN, lane);
+  } else {
+    // tile t of the MI NI of this output tile is wave t's to add up and store
+    static_assert(KW == 1 || (MI * NI == KW && MI * NI * 4096 <= RING && 32 * store_pitch<1, OUT>() <= RING), "a tile a wave");
     LDM_LOCKSTEP();
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int t = 0; t < MI * NI; ++t)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        reinterpret_cast<float4*>(ring)[(t * 4 + q) * 64 + lane] = make_float4(acc[t / NI][t % NI][4 * q], acc[t / NI][t % NI][4 * q + 1],
+                                                                               acc[t / NI][t % NI][4 * q + 2], acc[t / NI][t % NI][4 * q + 3]);
+    __syncthreads();
+    f32x16_t sum[1][1];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      float4 v = reinterpret_cast<const float4*>(smem)[(wave * 4 + q) * 64 + lane];
+#pragma unroll
+      for (int w = 1; w < KW; ++w) {
+        const float4 o = reinterpret_cast<const float4*>(smem + w * RING)[(wave * 4 + q) * 64 + lane];
+        v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+      }
+      sum[0][0][4 * q] = v.x; sum[0][0][4 * q + 1] = v.y; sum[0][0][4 * q + 2] = v.z; sum[0][0][4 * q + 3] = v.w;
+    }
+    __syncthreads();
+    store_tiles<1, 1, OUT>(p, sum, ring, m0 + wave / NI * 32, n0 + wave % NI * 32, lane);
   }
 }
 
@@ -559,6 +729,18 @@ static int launch_mx4_gemm(Mx4Params& p, hipStream_t st) {
   return LDM_OK;
 }
 
+template <int BM, int BN, int WM, int WN, int KW, int S, typename OUT>
+static int launch_bf16_gemm(Mx4Params& p, hipStream_t st) {
+  p.tiles_m = (int)((p.rows + BM - 1) / BM);
+  p.tiles_n = (p.n + BN - 1) / BN;
+  constexpr int smem = KW * S * (BM + BN) * 128;
+  auto kern = bf16_gemm_kernel<BM, BN, WM, WN, KW, S, OUT>;
+  static bool done = false;
+  if (int rc = mx_allow_lds("ldm_linear_bf16", kern, smem, done)) return rc;
+  hipLaunchKernelGGL(kern, dim3(p.tiles_m * p.tiles_n), dim3(64 * WM * WN * KW), smem, st, p);
+  return LDM_OK;
+}
+
 template <bool MX, int MT, int NF, int NW, int S, bool DMAX, typename OUT>
 static int launch_mx4_rows(const Mx4Params& p, hipStream_t st) {
   constexpr int smem = NW * (S * (NF + (MX ? MT : 4 * MT)) * 1024 + (MX ? 4096 : 2048));
@@ -598,6 +780,22 @@ static int mx4_linear_out(Mx4Params& p, bool mx, hipStream_t st) {
   return launch_mx4_gemm<128, 128, 2, 2, 4, true, OUT>(p, st);
 }
 
+template <typename OUT>
+static int linear_bf16_out(Mx4Params& p, hipStream_t st) {
+  // rounds of one workgroup a CU x the time of a step of the tile (us, measured at full chips: 64 x 64 with its columns split 0.27,
+  // 128 x 128 0.5, 128 x 160 0.7, 256 x 160 1.1).  8192 x 640 (k = 5120): 83 us with 128 x 128, 65 with 128 x 160; 32768 x 320 (k = 2560):
+  // 89, 77 and 62 with 256 x 160; 154 x 768 (k = 1312): 11.7 with 128 x 128, 6.8 with 64 x 64.
+  auto cost = [&](int bm, int bn, float step) {
+    const long long tiles = ((p.rows + bm - 1) / bm) * ((p.n + bn - 1) / bn);
+    return (float)((tiles + 255) / 256) * step;
+  };
+  const float a = cost(64, 64, 0.27f), b = cost(128, 128, 0.5f), c = cost(128, 160, 0.7f), d = cost(256, 160, 1.1f);
+  if (a <= b && a <= c && a <= d) return launch_bf16_gemm<64, 64, 1, 1, 4, 2, OUT>(p, st);
+  if (b <= c && b <= d) return launch_bf16_gemm<128, 128, 2, 2, 1, 3, OUT>(p, st);
+  if (c <= d) return launch_bf16_gemm<128, 160, 4, 1, 1, 3, OUT>(p, st);
+  return launch_bf16_gemm<256, 160, 4, 1, 1, 3, OUT>(p, st);
+}
+
 }  // namespace ldm
 
 using namespace ldm;
@@ -627,5 +825,23 @@ extern "C" int ldm_mx4_linear(const void* x, const void* x_scale, const void* w,
   const int rc = out_dtype == LDM_BF16 ? mx4_linear_out<bf16_t>(p, mx, st) : mx4_linear_out<float>(p, mx, st);
   if (rc) return rc;
   LDM_HIP_CHECK_LAUNCH("ldm_mx4_linear");
+  return LDM_OK;
+}
+
+extern "C" int ldm_linear_bf16(const void* x, const void* w, const float* bias, void* out, int out_dtype, long long rows, int n, int k, void* stream) {
+  LDM_REQUIRE(dtype_ok(out_dtype), "ldm_linear_bf16: bad dtype %d", out_dtype);
+  LDM_REQUIRE(rows >= 0 && n >= 1 && k >= 8 && k % 8 == 0 && k <= (1 << 21), "ldm_linear_bf16: bad sizes (rows=%lld n=%d k=%d; k a multiple of 8)",
+              rows, n, k);
+  if (rows == 0) return LDM_OK;
+  LDM_REQUIRE(x && w && out && aligned16(x) && aligned16(w) && (reinterpret_cast<uintptr_t>(bias) & 3) == 0 &&
+                  reinterpret_cast<uintptr_t>(out) % dtype_size(out_dtype) == 0,
+              "ldm_linear_bf16: null or unaligned pointer");
+  Mx4Params p{};
+  p.x = static_cast<const unsigned char*>(x); p.w = static_cast<const unsigned char*>(w);
+  p.bias = bias; p.out = out; p.rows = rows; p.n = n; p.k = k;
+  p.nk = (k + 63) / 64;
+  const int rc = out_dtype == LDM_BF16 ? linear_bf16_out<bf16_t>(p, (hipStream_t)stream) : linear_bf16_out<float>(p, (hipStream_t)stream);
+  if (rc != LDM_OK) return rc;
+  LDM_HIP_CHECK_LAUNCH("ldm_linear_bf16");
   return LDM_OK;
 }

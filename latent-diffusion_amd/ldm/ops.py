@@ -1072,11 +1072,20 @@ _MX4_WIDEN_ROWS = 64        # bf16 activations: up to here the weights are widen
 
 
 def _pad_cols(t: torch.Tensor, cols: int) -> torch.Tensor:
-    """(rows, c) -> (rows, cols) zero-padded copy (t itself if it has them): operands of the implicit GEMM come in whole 32 columns."""
-    if t.shape[-1] == cols:
+    """(rows, c) -> (rows, cols) zero-padded copy for operands that are fetched 16 bytes at a time; t itself if it can be."""
+    if t.shape[-1] == cols and t.data_ptr() % 16 == 0:
         return t
     out = torch.zeros((t.shape[0], cols), dtype=t.dtype, device=t.device)
     out[:, :t.shape[-1]] = t
+    return out
+
+
+def _linear_bf16(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], out_dtype: torch.dtype) -> torch.Tensor:
+    """x (rows, k) W^T + bias for widened weights w (n, k rounded up to 8)."""
+    rows, (n, kp) = x.shape[0], w.shape
+    x = _pad_cols(x, kp)
+    out = torch.empty((rows, n), dtype=out_dtype, device=x.device)
+    _call(x, "ldm_linear_bf16", x.data_ptr(), w.data_ptr(), _ptr(bias), out.data_ptr(), dt_code(out_dtype), rows, n, kp)
     return out
 
 
@@ -1109,10 +1118,10 @@ def mx4_linear(x, w: MxTensor, bias: Optional[torch.Tensor] = None, out_dtype: O
     rows = xt.numel() // xt.shape[-1]
     if not mx and rows > _MX4_WIDEN_ROWS:
         # many rows: the weights are read by many workgroups, so widening them once costs less than in every one of them
-        kp = (k + 31) // 32 * 32
+        kp = (k + 7) // 8 * 8
         wide = torch.empty((n, kp), dtype=torch.bfloat16, device=x.device)
         _call(x, "ldm_mx_dequantize", w.data.data_ptr(), w.scale.data_ptr(), _lib.MX4, n, kp, wide.data_ptr(), BF16, kp)
-        return conv_gemm(_pad_cols(x.reshape(rows, k), kp), wide, bias=bias, out_dtype=odt).view(*lead, n)
+        return _linear_bf16(x.reshape(rows, k), wide, bias, odt).view(*lead, n)
     out = torch.empty((*lead, n), dtype=odt, device=xt.device)
     if rows:
         _call(xt, "ldm_mx4_linear", xt.data_ptr(), x.scale.data_ptr() if mx else 0, w.data.data_ptr(), w.scale.data_ptr(), _ptr(bias),
@@ -1136,10 +1145,10 @@ def mx4_linear_dgrad(dy: torch.Tensor, w: MxTensor) -> torch.Tensor:
     rows = dy.numel() // n
     if rows == 0:
         return torch.empty((*dy.shape[:-1], k), dtype=dy.dtype, device=dy.device)
-    np_ = (n + 31) // 32 * 32
+    np_ = (n + 7) // 8 * 8
     wt = torch.empty((k, np_), dtype=torch.bfloat16, device=dy.device)
     _call(dy, "ldm_mx4_dequantize_t", w.data.data_ptr(), w.scale.data_ptr(), n, k, wt.data_ptr(), np_)
-    return conv_gemm(_pad_cols(dy.reshape(rows, n), np_), wt).view(*dy.shape[:-1], k)
+    return _linear_bf16(dy.reshape(rows, n), wt, None, torch.bfloat16).view(*dy.shape[:-1], k)
 
 
 def _glu_kind(what: str, act: str) -> int:
