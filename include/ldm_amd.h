@@ -452,6 +452,10 @@ int ldm_glu_backward_mx8(const void* data, const void* scale, const void* dout, 
 int ldm_mx4_linear(const void* x, const void* x_scale, const void* w, const void* w_scale, const float* bias, void* out, int out_dtype,
                    long long rows, int n, int k, void* stream);
 
+/* out (rows, ld) bfloat16 = x (rows, cols), contiguous at any alignment, zeros behind; ld a multiple of 8, out 16-byte aligned: rows for
+ * the operators that fetch 16 bytes at a time. */
+int ldm_pad_columns_bf16(const void* x, void* out, long long rows, int cols, int ld, void* stream);
+
 /* out (rows, n) = x W^T + bias for plain bfloat16 operands x (rows, k), w (n, k), contiguous, 16-byte aligned, k a multiple of 8 up to
  * 2^21: the product behind ldm_mx_dequantize / ldm_mx4_dequantize_t, for many rows.  bias, out, sums as above. */
 int ldm_linear_bf16(const void* x, const void* w, const float* bias, void* out, int out_dtype, long long rows, int n, int k, void* stream);

@@ -268,6 +268,27 @@ mx4_dequantize_t_kernel(const unsigned char* __restrict__ data, const unsigned c
   }
 }
 
+// ------------------------------------------------------------------------------------------------------------------ pad
+// rows of `cols` bf16 -> rows of ld (a multiple of 8), zeros behind: 16 bytes a thread, one pass (a clear and a copy would be two)
+__global__ void __launch_bounds__(256)
+pad_columns_kernel(const bf16_t* __restrict__ x, bf16_t* __restrict__ out, long long rows, int cols, int ld) {
+  const int c = (blockIdx.x * 256 + threadIdx.x) * 8;
+  if (c >= ld) return;
+  for (long long r = blockIdx.y; r < rows; r += gridDim.y) {
+    const bf16_t* src = x + r * cols + c;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (c + 8 <= cols) {
+      v = load16_any(src);
+    } else {
+      uint32_t h[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) h[e] = c + e < cols ? src[e] : 0;
+      v = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+    }
+    *reinterpret_cast<uint4*>(out + r * ld + c) = v;
+  }
+}
+
 // --------------------------------------------------------------------------------------------------- gated activation
 // h: (rows, 2 ff) with columns in the paired order of ldm_pack_weight(glu_pairs): blocks of 16 values, then their 16 gates -- an mx8
 // block is exactly one such pair of blocks, so two threads hold a block: each 8 values and their 8 gates.
@@ -483,6 +504,17 @@ extern "C" int ldm_mx4_dequantize_t(const void* data, const void* scale, int row
                      static_cast<const unsigned char*>(data), static_cast<const unsigned char*>(scale), static_cast<bf16_t*>(out), rows, cols,
                      mx_blocks(cols), mx_scale_stride(cols), ld);
   LDM_HIP_CHECK_LAUNCH("ldm_mx4_dequantize_t");
+  return LDM_OK;
+}
+
+extern "C" int ldm_pad_columns_bf16(const void* x, void* out, long long rows, int cols, int ld, void* stream) {
+  LDM_REQUIRE(rows >= 0 && cols >= 1 && ld >= cols && ld % 8 == 0 && ld <= (1 << 30), "ldm_pad_columns_bf16: bad sizes (rows=%lld cols=%d ld=%d)", rows,
+              cols, ld);
+  if (rows == 0) return LDM_OK;
+  LDM_REQUIRE(x && out && aligned16(out) && (reinterpret_cast<uintptr_t>(x) & 1) == 0, "ldm_pad_columns_bf16: null or unaligned pointer");
+  hipLaunchKernelGGL(pad_columns_kernel, dim3((ld / 8 + 255) / 256, (unsigned)(rows < 65535 ? rows : 65535)), dim3(256), 0, (hipStream_t)stream,
+                     static_cast<const bf16_t*>(x), static_cast<bf16_t*>(out), rows, cols, ld);
+  LDM_HIP_CHECK_LAUNCH("ldm_pad_columns_bf16");
   return LDM_OK;
 }
 

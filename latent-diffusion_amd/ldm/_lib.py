@@ -128,6 +128,7 @@ _SIGNATURES = {
     "ldm_glu_forward_mx8": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, C.c_longlong, c_int, c_int, c_void_p],
     "ldm_glu_backward_mx8": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, C.c_longlong, c_int, c_int, c_void_p],
     "ldm_mx4_linear": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, C.c_longlong, c_int, c_int, c_void_p],
+    "ldm_pad_columns_bf16": [c_void_p, c_void_p, C.c_longlong, c_int, c_int, c_void_p],
     "ldm_linear_bf16": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, C.c_longlong, c_int, c_int, c_void_p],
     "ldm_linear_wgrad_mx8": [c_void_p, c_void_p, c_void_p, c_void_p, C.c_longlong, c_int, c_int, c_int, c_void_p, C.c_longlong,
                              c_void_p],

@@ -1072,11 +1072,11 @@ _MX4_WIDEN_ROWS = 64        # bf16 activations: up to here the weights are widen
 
 
 def _pad_cols(t: torch.Tensor, cols: int) -> torch.Tensor:
-    """(rows, c) -> (rows, cols) zero-padded copy for operands that are fetched 16 bytes at a time; t itself if it can be."""
+    """bfloat16 (rows, c) -> (rows, cols) zero-padded copy for operands that are fetched 16 bytes at a time; t itself if it can be."""
     if t.shape[-1] == cols and t.data_ptr() % 16 == 0:
         return t
-    out = torch.zeros((t.shape[0], cols), dtype=t.dtype, device=t.device)
-    out[:, :t.shape[-1]] = t
+    out = torch.empty((t.shape[0], cols), dtype=t.dtype, device=t.device)
+    _call(t, "ldm_pad_columns_bf16", t.data_ptr(), out.data_ptr(), t.shape[0], t.shape[1], cols)
     return out
 
 
