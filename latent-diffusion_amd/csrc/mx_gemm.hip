@@ -61,6 +61,7 @@ __device__ __forceinline__ void lds_read4(int& v, unsigned addr) {
 }
 // no use of v moves above the wait in front of this
 __device__ __forceinline__ void stay_below(i32x4_t& v) { asm volatile("" : "+v"(v)); }
+__device__ __forceinline__ void stay_below(int& v) { asm volatile("" : "+v"(v)); }
 
 template <bool MX, int H>
 __device__ __forceinline__ void mx_mfma(f32x16_t& c, i32x4_t a, i32x4_t b, int sa, int sb) {
@@ -133,8 +134,8 @@ __device__ __forceinline__ void store_tiles(const Mx4Params& p, const f32x16_t (
   }
 }
 
-// Tile of BM (rows of x) x BN (rows of w) by WM x WN waves; a step is 64 bytes of every row (MX: 128 columns of mx4, four blocks; else 32
-// columns of bf16), S slots of LDS.  16-byte chunks of a row are XOR-swizzled by (row >> 1) & 3 (the DMA writes lane-linear, so the
+// Large products: tile of BM (rows of x) x BN (rows of w) by WM x WN waves; a step is 64 bytes of every row (128 columns of mx4, four
+// blocks), S slots of LDS.  16-byte chunks of a row are XOR-swizzled by (row >> 1) & 3 (the DMA writes lane-linear, so the
 // swizzle is applied to the lane's SOURCE chunk and again on the read): eight consecutive rows then lie in eight different 16-byte
 // columns of the 128-byte LDS line.  A chunk is what a lane gives one matrix instruction -- a block, or 8 columns of bf16 -- so
 // chunks past the end of a row are fetched from beyond the descriptor's end (zeros), and rows past the end likewise.
@@ -145,15 +146,15 @@ __device__ __forceinline__ void store_tiles(const Mx4Params& p, const f32x16_t (
 //
 // Scales: one 32-bit word a row and step.  From four steps on, 16 bytes (four steps) a row at a time in one DMA instruction, the last
 // ones ending with the row (a fetch never passes its row); with fewer steps word by word, once.
-template <int BM, int BN, int WM, int WN, int S, bool MX, typename OUT>
-__global__ void __launch_bounds__(64 * WM * WN, 2)
+template <int BM, int BN, int WM, int WN, int S, typename OUT>
+__global__ void __launch_bounds__(64 * WM * WN)
 mx4_gemm_kernel(const Mx4Params p) {
   constexpr int NT = 64 * WM * WN, ROWS = BM + BN;
   constexpr int IT = ROWS * 4 / NT;                        // tile DMA instructions of a wave a step
   constexpr int SIT = ROWS / NT;                           // scale DMA instructions of a wave (16 bytes a row)
   static_assert(BM * 4 % NT == 0 && BN * 4 % NT == 0 && ROWS % NT == 0 && BM % 64 == 0, "tile / threads mismatch");
   constexpr int STAGE = ROWS * 64;
-  constexpr int SCALES = MX ? ROWS * 16 : 0;               // one group of four steps
+  constexpr int SCALES = ROWS * 16;              // one group of four steps
   constexpr int WTM = BM / WM, WTN = BN / WN, MI = WTM / 32, NI = WTN / 32;
   constexpr unsigned OOB = 0x80000000u;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -172,7 +173,7 @@ mx4_gemm_kernel(const Mx4Params p) {
   const long long m0 = (long long)tm * BM;
   const int n0 = tn * BN;
 
-  const int rb = MX ? p.blocks * 16 : p.k * 2, chunks = rb >> 4;
+  const int rb = p.blocks * 16;
   const int mrows = (int)min((long long)BM, p.rows - m0), nrows = min(BN, p.n - n0);
   const unsigned char* xbase = p.x + m0 * rb;
   const unsigned char* wbase = p.w + (long long)n0 * rb;
@@ -218,10 +219,9 @@ mx4_gemm_kernel(const Mx4Params p) {
   };
   // a step past the last one is fetched like any other (zeros, into a slot that nobody reads): the loop needs no case for its end
   auto stage = [&](int kt) {
-    if constexpr (MX)
-      if ((kt & 3) == 0 && kt < nk) stage_scales(kt >> 2);
+    if ((kt & 3) == 0 && kt < nk) stage_scales(kt >> 2);
     unsigned char* dst = smem + (kt % S) * STAGE + wave * 1024;
-    const bool past = kt * 4 + chunk >= chunks;
+    const bool past = kt * 4 + chunk >= p.blocks;
 #pragma unroll
     for (int it = 0; it < IT; ++it) {                      // 16 whole rows a wave and instruction, all of one operand
       const unsigned vo = past ? OOB : voff[it];
@@ -260,15 +260,13 @@ mx4_gemm_kernel(const Mx4Params p) {
     else lds_read16<j * 2048>(wf[H][j], (waddr ^ (H * 32)) + slot);
   };
   auto read_scales = [&](int kt) {
-    if constexpr (MX) {
-      const int g = kt >> 2, word = kt - group_first(g);
-      const unsigned o = (g & 1) * SCALES + word * (word_scales ? ROWS * 4 : 4);
-      const unsigned step = 32 * sstep;
+    const int g = kt >> 2, word = kt - group_first(g);
+    const unsigned o = (g & 1) * SCALES + word * (word_scales ? ROWS * 4 : 4);
+    const unsigned step = 32 * sstep;
 #pragma unroll
-      for (int i = 0; i < MI; ++i) lds_read4<0>(nsx[i], xsaddr + o + i * step);
+    for (int i = 0; i < MI; ++i) lds_read4<0>(nsx[i], xsaddr + o + i * step);
 #pragma unroll
-      for (int j = 0; j < NI; ++j) lds_read4<0>(nsw[j], wsaddr + o + j * step);
-    }
+    for (int j = 0; j < NI; ++j) lds_read4<0>(nsw[j], wsaddr + o + j * step);
   };
   auto landed = [&]<int H>(std::integral_constant<int, H>) {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -276,7 +274,7 @@ mx4_gemm_kernel(const Mx4Params p) {
     for (int i = 0; i < MI; ++i) asm volatile("" : "+v"(xf[H][i]));   // no use moves above the wait
 #pragma unroll
     for (int j = 0; j < NI; ++j) asm volatile("" : "+v"(wf[H][j]));
-    if constexpr (MX && H == 0) {
+    if constexpr (H == 0) {
 #pragma unroll
       for (int i = 0; i < MI; ++i) { asm volatile("" : "+v"(nsx[i])); sx[i] = (int)((unsigned)nsx[i] >> (8 * fh)); }
 #pragma unroll
@@ -288,7 +286,7 @@ mx4_gemm_kernel(const Mx4Params p) {
     [&]<int... Q>(std::integer_sequence<int, Q...>) {
       ([&] {
         constexpr int q = Q, i = q / NI, j = q % NI;
-        mx_mfma<MX, H>(acc[i][j], wf[H][j], xf[H][i], sw[j], sx[i]);
+        mx_mfma<true, H>(acc[i][j], wf[H][j], xf[H][i], sw[j], sx[i]);
         if constexpr (q < READS) read(std::integral_constant<int, 1 - H>{}, std::integral_constant<int, q>{}, slot);
         __builtin_amdgcn_sched_barrier(0);
       }(), ...);
@@ -330,26 +328,35 @@ mx4_gemm_kernel(const Mx4Params p) {
   store_tiles<MI, NI, OUT>(p, acc, smem + wave * 32 * store_pitch<NI, OUT>(), m0 + wm * WTM, n0 + wn * WTN, lane);
 }
 
-// ------------------------------------------------------------------------------------------------- plain bf16 operands
-// out = x W^T + bias for bf16 rows: the product behind the widening of the weights.  A step is 64 columns (128 bytes) of every row: the
-// chip's L2 hands out lines of 128 bytes, and LDS-DMA of 64 of them a row gets half the rate (17 against 29 TB/s over all CUs).  Chunks
-// are swizzled by row & 7.  The registers of a whole step -- four rounds of v_mfma_f32_32x32x16_bf16 -- are read while the step before
-// multiplies, one barrier a step.  What bounds the loop is LDS: a wave's tile of 64 x 64 reads as many bytes as its instructions take
-// time, 32 x 160 and 64 x 160 fewer.
-//   KW == 1: WM x WN waves share a tile of BM x BN.
+// Tile of BM (rows of x) x BN (rows of w).  A step is 128 bytes of every row (MX: 256 columns of mx4, eight blocks; else 64 columns of
+// bf16): the chip's L2 hands out lines of 128 bytes, and LDS-DMA of 64 of them a row gets half the rate (17 against 29 TB/s over all CUs).
+// 16-byte chunks of a row are XOR-swizzled by row & 7 (the DMA writes lane-linear, so the swizzle is applied to the lane's SOURCE chunk
+// and again on the read): eight consecutive rows then lie in eight different 16-byte columns of LDS.  A chunk is what a lane gives one
+// matrix instruction -- a block, or 8 columns of bf16 -- so chunks past the end of a row are fetched from beyond the descriptor's end
+// (zeros), rows past the end likewise, and steps past the end too: their number is rounded up to an even one.
+//
+// S slots of LDS.  The registers of a whole step -- four rounds of matrix instructions -- are read while the step before multiplies, reads and
+// DMA spread between the instructions, one barrier a step.  What bounds the loop is LDS: a wave's tile of 64 x 64 reads as many bytes as its
+// instructions take time, 64 x 128 or 64 x 160 fewer.
+//   KW == 1: WM x WN waves share the tile.
 //   KW > 1:  few tiles, where a launch is as long as one workgroup's chain of steps: the KW waves of a workgroup each take a contiguous part
 //            of the columns of the whole tile, with a ring of their own and no barrier, and add up through LDS in a fixed order.
-// Steps past the end are fetched as zeros, so the number of steps is rounded up to an even one.
-template <int BM, int BN, int WM, int WN, int KW, int S, typename OUT>
+//
+// Scales (MX): two 32-bit words a row and step.  From four words a row on, 16 bytes (two steps) a row at a time in one DMA instruction, the
+// last ones ending with the row (a fetch never passes its row); with fewer words one by one, once.  Words past the end count as zero: what
+// LDS holds there may be another row's NaN.
+template <int BM, int BN, int WM, int WN, int KW, int S, bool MX, typename OUT>
 __global__ void __launch_bounds__(64 * WM * WN * KW, KW > 1 || BM * BN > 16384 ? 1 : 2)
-bf16_gemm_kernel(const Mx4Params p) {
+mx_gemm_kernel(const Mx4Params p) {
   static_assert(KW == 1 || (WM == 1 && WN == 1), "a wave of its own tile or of its own columns");
   constexpr int NT = 64 * WM * WN, ROWS = BM + BN;
   constexpr int IT = ROWS * 8 / NT;                        // DMA instructions of a wave a step
-  constexpr int STAGE = ROWS * 128, RING = S * STAGE;
+  constexpr int STAGE = ROWS * 128;
+  constexpr int SROWS = (ROWS + 63) / 64 * 64, SCALES = MX ? SROWS * 16 : 0;   // one group of two steps
+  constexpr int RING = S * STAGE + 2 * SCALES;
   constexpr int WTM = BM / WM, WTN = BN / WN, MI = WTM / 32, NI = WTN / 32;
   constexpr unsigned OOB = 0x80000000u;
-  static_assert(BM * 8 % NT == 0 && BN * 8 % NT == 0 && (S - 2) * IT < 64, "tile / threads mismatch");
+  static_assert(BM * 8 % NT == 0 && BN * 8 % NT == 0 && BM % 64 == 0 && (S - 2) * IT < 64, "tile / threads mismatch");
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
 
   const int tid = threadIdx.x, lane = tid & 63;
@@ -360,21 +367,46 @@ bf16_gemm_kernel(const Mx4Params p) {
   const int fr = lane & 31, fh = lane >> 5;
 
   const int tile = mx_xcd_remap(blockIdx.x, gridDim.x);
+  // bands of 4 tile rows walked column by column: the tiles in flight on one XCD share their operands in its L2
   const int band = 4 * p.tiles_n, g4 = tile / band, in = tile - g4 * band;
   const int brows = min(p.tiles_m - g4 * 4, 4);
   const int tn = in / brows, tm = g4 * 4 + (in - tn * brows);
   const long long m0 = (long long)tm * BM;
   const int n0 = tn * BN;
 
-  const int rb = p.k * 2, chunks = p.k >> 3;
+  const int rb = MX ? p.blocks * 16 : p.k * 2, chunks = rb >> 4;
+  const int mrows = (int)min((long long)BM, p.rows - m0), nrows = min(BN, p.n - n0);
   const unsigned char* xbase = p.x + m0 * rb;
   const unsigned char* wbase = p.w + (long long)n0 * rb;
-  const unsigned xbytes = (unsigned)min((long long)BM, p.rows - m0) * rb, wbytes = (unsigned)min(BN, p.n - n0) * rb;
+  const unsigned xbytes = (unsigned)mrows * rb, wbytes = (unsigned)nrows * rb;
   const int chunk = (gt & 7) ^ ((gt >> 3) & 7);
   const unsigned voff = (unsigned)(gt >> 3) * rb + chunk * 16;
 
   const int per = ((p.nk + KW - 1) / KW + 1) & ~1, s0 = kw * per;
   unsigned char* const ring = smem + kw * RING;
+
+  const int nwords = p.sstride >> 2;                       // scale words a row
+  const bool word_scales = nwords < 4;
+  // word w of row r of group g lies at group + r * row_step + (w - first word of the group) * word_step
+  auto group_first = [&](int kt) { return word_scales ? 0 : min((s0 + (kt & ~1)) * 2, nwords - 4); };
+  auto stage_scales = [&](int kt) {                        // of steps kt and kt + 1, kt even
+    unsigned char* dst = ring + S * STAGE + ((kt >> 1) & 1) * SCALES;
+    const unsigned char* xs = p.xs + m0 * p.sstride;
+    const unsigned char* ws = p.ws + (long long)n0 * p.sstride;
+    const unsigned xsb = (unsigned)mrows * p.sstride, wsb = (unsigned)nrows * p.sstride;
+#pragma unroll
+    for (int it = 0; it < (SROWS + NT - 1) / NT; ++it) {
+      const int r0 = it * NT + gw * 64;
+      if (r0 >= SROWS) continue;
+      const bool isx = r0 < BM;
+      const unsigned vo = (unsigned)(r0 - (isx ? 0 : BM) + lane) * p.sstride;
+      if (word_scales) {
+        for (int j = 0; j < nwords; ++j) mx_dma4(isx ? xs : ws, isx ? xsb : wsb, dst + (j * SROWS + r0) * 4, vo, j * 4);
+      } else {
+        mx_dma16(isx ? xs : ws, isx ? xsb : wsb, dst + r0 * 16, vo, group_first(kt) * 4);
+      }
+    }
+  };
   auto stage_part = [&](int kt, int it) {                  // instruction `it` of step s0 + kt
     unsigned char* dst = ring + (kt % S) * STAGE + gw * 1024 + it * NT * 16;
     const bool past = kt >= per || (s0 + kt) * 8 + chunk >= chunks;
@@ -382,7 +414,12 @@ bf16_gemm_kernel(const Mx4Params p) {
     if (it * NT < BM * 8) mx_dma16(xbase, xbytes, dst, past ? OOB : voff + it * (NT / 8) * rb, so);
     else mx_dma16(wbase, wbytes, dst, past ? OOB : voff + (it * (NT / 8) - BM) * rb, so);
   };
+  auto stage_begin = [&](int kt) {
+    if constexpr (MX)
+      if ((kt & 1) == 0 && kt < per) stage_scales(kt);
+  };
   auto stage = [&](int kt) {
+    stage_begin(kt);
 #pragma unroll
     for (int it = 0; it < IT; ++it) stage_part(kt, it);
   };
@@ -396,16 +433,41 @@ bf16_gemm_kernel(const Mx4Params p) {
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 
   i32x4_t xf[2][4][MI], wf[2][4][NI];                      // [set][round of the step]
+  // scale words of rounds 0, 1 and 2, 3: as read, and shifted so that byte 0 / byte 2 is this lane's block of the even / odd round
+  int rx[2][MI], rw[2][NI], sx[2][MI], sw[2][NI];
+#pragma unroll
+  for (int o = 0; o < 2; ++o) {
+#pragma unroll
+    for (int i = 0; i < MI; ++i) rx[o][i] = sx[o][i] = 0;
+#pragma unroll
+    for (int j = 0; j < NI; ++j) rw[o][j] = sw[o][j] = 0;
+  }
   const unsigned lds = (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)ring;
   const int swz = fr & 7;
   const unsigned xaddr = lds + (wm * WTM + fr) * 128 + ((fh ^ swz) << 4), waddr = lds + (BM + wn * WTN + fr) * 128 + ((fh ^ swz) << 4);
   constexpr int READS = 4 * (MI + NI), MM = 4 * MI * NI;
+  static_assert(READS <= 2 * MM, "every read has its place");
   auto read = [&]<int SET, int Q>(std::integral_constant<int, SET>, std::integral_constant<int, Q>, unsigned slot) {
     constexpr int h = Q / (MI + NI), q = Q % (MI + NI), i = q < MI ? q : 0, j = q < MI ? 0 : q - MI;
     if constexpr (q < MI) lds_read16<i * 4096>(xf[SET][h][i], (xaddr ^ (h * 32)) + slot);
     else lds_read16<j * 4096>(wf[SET][h][j], (waddr ^ (h * 32)) + slot);
   };
-  auto landed = [&]<int SET>(std::integral_constant<int, SET>) {
+  const int row_step = word_scales ? 4 : 16, word_step = word_scales ? SROWS * 4 : 4;
+  auto read_scales = [&](int kt) {
+    if constexpr (MX) {
+      const unsigned base = lds + S * STAGE + ((kt >> 1) & 1) * SCALES;
+      const int w = (s0 + kt) * 2 - group_first(kt);
+#pragma unroll
+      for (int o = 0; o < 2; ++o) {
+        const unsigned at = base + min(w + o, 3) * word_step;
+#pragma unroll
+        for (int i = 0; i < MI; ++i) lds_read4<0>(rx[o][i], at + (wm * WTM + i * 32 + fr) * row_step);
+#pragma unroll
+        for (int j = 0; j < NI; ++j) lds_read4<0>(rw[o][j], at + (BM + wn * WTN + j * 32 + fr) * row_step);
+      }
+    }
+  };
+  auto landed = [&]<int SET>(std::integral_constant<int, SET>, int kt) {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
     for (int h = 0; h < 4; ++h) {
@@ -414,44 +476,54 @@ bf16_gemm_kernel(const Mx4Params p) {
 #pragma unroll
       for (int j = 0; j < NI; ++j) stay_below(wf[SET][h][j]);
     }
+    if constexpr (MX) {
+#pragma unroll
+      for (int o = 0; o < 2; ++o) {
+        const unsigned there = (s0 + kt) * 2 + o < nwords ? ~0u : 0u;
+#pragma unroll
+        for (int i = 0; i < MI; ++i) { stay_below(rx[o][i]); sx[o][i] = (int)(((unsigned)rx[o][i] & there) >> (8 * fh)); }
+#pragma unroll
+        for (int j = 0; j < NI; ++j) { stay_below(rw[o][j]); sw[o][j] = (int)(((unsigned)rw[o][j] & there) >> (8 * fh)); }
+      }
+    }
   };
   auto next_here = [&] {                                   // the next step's DMA has landed, and the slot of this one is free
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 2) * IT) : "memory");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 2) * IT) : "memory");   // a fetch of scales behind it only makes the wait stricter
     if constexpr (KW == 1) __builtin_amdgcn_s_barrier();
     else LDM_LOCKSTEP();
     asm volatile("" ::: "memory");
   };
-  // step kt from register set SET; the next one's reads between the matrix instructions
+  // step kt from register set SET; the next one's reads, and the DMA into the slot that is free now, between the matrix instructions
   auto step = [&]<int SET>(std::integral_constant<int, SET>, int kt) {
     next_here();
+    stage_begin(kt + S);
+    read_scales(kt + 1);
     const unsigned slot = (unsigned)((kt + 1) % S) * STAGE;
     [&]<int... Q>(std::integer_sequence<int, Q...>) {
       ([&] {
         constexpr int q = Q, h = q / (MI * NI), i = q / NI % MI, j = q % NI;
-        mx_mfma<false, h>(acc[i][j], wf[SET][h][j], xf[SET][h][i], 0, 0);
-        // two reads at a time: all are out by the middle of the step
+        mx_mfma<MX, h & 1>(acc[i][j], wf[SET][h][j], xf[SET][h][i], sw[h >> 1][j], sx[h >> 1][i]);
         if constexpr (2 * q < READS) read(std::integral_constant<int, 1 - SET>{}, std::integral_constant<int, 2 * q>{}, slot);
         if constexpr (2 * q + 1 < READS) read(std::integral_constant<int, 1 - SET>{}, std::integral_constant<int, 2 * q + 1>{}, slot);
-        // the DMA spread likewise: issued in one go it holds the wave up for as long as it takes
 #pragma unroll
         for (int it = q * IT / MM; it < (q + 1) * IT / MM; ++it) stage_part(kt + S, it);
         __builtin_amdgcn_sched_barrier(0);
       }(), ...);
     }(std::make_integer_sequence<int, MM>{});
-    landed(std::integral_constant<int, 1 - SET>{});
+    landed(std::integral_constant<int, 1 - SET>{}, kt + 1);
   };
   constexpr std::integral_constant<int, 0> SET0{};
   constexpr std::integral_constant<int, 1> SET1{};
-  static_assert(READS <= 2 * MM, "every read has its place");
 
 #pragma unroll
   for (int t = 0; t < S - 1; ++t) stage(t);
   next_here();
   stage(S - 1);
+  read_scales(0);
   [&]<int... Q>(std::integer_sequence<int, Q...>) {
     (read(SET0, std::integral_constant<int, Q>{}, 0u), ...);
   }(std::make_integer_sequence<int, READS>{});
-  landed(SET0);
+  landed(SET0, 0);
   for (int kt = 0; kt < per; kt += 2) {
     step(SET0, kt);
     step(SET1, kt + 1);
@@ -717,26 +789,29 @@ static int mx_allow_lds(const char* what, K kern, int bytes, bool& done) {
   return LDM_OK;
 }
 
-template <int BM, int BN, int WM, int WN, int S, bool MX, typename OUT>
+template <int BM, int BN, int WM, int WN, int S, typename OUT>
 static int launch_mx4_gemm(Mx4Params& p, hipStream_t st) {
   p.tiles_m = (int)((p.rows + BM - 1) / BM);
   p.tiles_n = (p.n + BN - 1) / BN;
-  constexpr int smem = (BM + BN) * (S * 64 + (MX ? 2 * 16 : 0));
-  auto kern = mx4_gemm_kernel<BM, BN, WM, WN, S, MX, OUT>;
+  p.nk = (p.blocks + 3) / 4;
+  constexpr int smem = (BM + BN) * (S * 64 + 2 * 16);
+  auto kern = mx4_gemm_kernel<BM, BN, WM, WN, S, OUT>;
   static bool done = false;
   if (int rc = mx_allow_lds("ldm_mx4_linear", kern, smem, done)) return rc;
   hipLaunchKernelGGL(kern, dim3(p.tiles_m * p.tiles_n), dim3(64 * WM * WN), smem, st, p);
   return LDM_OK;
 }
 
-template <int BM, int BN, int WM, int WN, int KW, int S, typename OUT>
-static int launch_bf16_gemm(Mx4Params& p, hipStream_t st) {
+template <int BM, int BN, int WM, int WN, int KW, int S, bool MX, typename OUT>
+static int launch_mx_gemm(Mx4Params& p, hipStream_t st) {
   p.tiles_m = (int)((p.rows + BM - 1) / BM);
   p.tiles_n = (p.n + BN - 1) / BN;
-  constexpr int smem = KW * S * (BM + BN) * 128;
-  auto kern = bf16_gemm_kernel<BM, BN, WM, WN, KW, S, OUT>;
+  p.nk = (MX ? p.blocks + 7 : p.k / 8 + 7) / 8;
+  constexpr int smem = KW * (S * (BM + BN) * 128 + (MX ? 2 * ((BM + BN + 63) / 64 * 64) * 16 : 0));
+  static_assert(smem <= 160 * 1024, "LDS of a CU");
+  auto kern = mx_gemm_kernel<BM, BN, WM, WN, KW, S, MX, OUT>;
   static bool done = false;
-  if (int rc = mx_allow_lds("ldm_linear_bf16", kern, smem, done)) return rc;
+  if (int rc = mx_allow_lds("mx product", kern, smem, done)) return rc;
   hipLaunchKernelGGL(kern, dim3(p.tiles_m * p.tiles_n), dim3(64 * WM * WN * KW), smem, st, p);
   return LDM_OK;
 }
@@ -771,13 +846,20 @@ static int rows_by_size(const Mx4Params& p, hipStream_t st) {
   return launch_mx4_rows<MX, 4, 2, 4, MX ? 4 : 2, DMAX, OUT>(p, st);
 }
 
+static float tile_rounds(const Mx4Params& p, int bm, int bn) {
+  return (float)((((p.rows + bm - 1) / bm) * ((p.n + bn - 1) / bn) + 255) / 256);
+}
+
 template <typename OUT>
 static int mx4_linear_out(Mx4Params& p, bool mx, hipStream_t st) {
   if (!mx) return p.k % 8 == 0 && aligned16(p.x) ? rows_by_size<false, true, OUT>(p, st) : rows_by_size<false, false, OUT>(p, st);
   if (p.rows <= 64) return rows_by_size<true, true, OUT>(p, st);
-  const long long tiles = ((p.rows + 255) / 256) * ((p.n + 255) / 256);
-  if (tiles >= 128) return launch_mx4_gemm<256, 256, 2, 4, 4, true, OUT>(p, st);
-  return launch_mx4_gemm<128, 128, 2, 2, 4, true, OUT>(p, st);
+  // rounds of one workgroup a CU x the time of 256 columns of the tile (us: 64 x 64 with its columns split 0.55, 128 x 128 1, 256 x 256
+  // 2.3).  8192^3: 715, 464 and 341 us; 2048^3: 21.5, 11.5, 12.3; 154 x 2560 (k = 2560): 7.3, 10.4, 12.0
+  const float a = tile_rounds(p, 64, 64) * 0.55f, b = tile_rounds(p, 128, 128), c = tile_rounds(p, 256, 256) * 2.3f;
+  if (a <= b && a <= c) return launch_mx_gemm<64, 64, 1, 1, 4, 2, true, OUT>(p, st);
+  if (b <= c) return launch_mx_gemm<128, 128, 2, 2, 1, 3, true, OUT>(p, st);
+  return launch_mx4_gemm<256, 256, 2, 4, 4, OUT>(p, st);
 }
 
 template <typename OUT>
@@ -785,15 +867,12 @@ static int linear_bf16_out(Mx4Params& p, hipStream_t st) {
   // rounds of one workgroup a CU x the time of a step of the tile (us, measured at full chips: 64 x 64 with its columns split 0.27,
   // 128 x 128 0.5, 128 x 160 0.7, 256 x 160 1.1).  8192 x 640 (k = 5120): 83 us with 128 x 128, 65 with 128 x 160; 32768 x 320 (k = 2560):
   // 89, 77 and 62 with 256 x 160; 154 x 768 (k = 1312): 11.7 with 128 x 128, 6.8 with 64 x 64.
-  auto cost = [&](int bm, int bn, float step) {
-    const long long tiles = ((p.rows + bm - 1) / bm) * ((p.n + bn - 1) / bn);
-    return (float)((tiles + 255) / 256) * step;
-  };
-  const float a = cost(64, 64, 0.27f), b = cost(128, 128, 0.5f), c = cost(128, 160, 0.7f), d = cost(256, 160, 1.1f);
-  if (a <= b && a <= c && a <= d) return launch_bf16_gemm<64, 64, 1, 1, 4, 2, OUT>(p, st);
-  if (b <= c && b <= d) return launch_bf16_gemm<128, 128, 2, 2, 1, 3, OUT>(p, st);
-  if (c <= d) return launch_bf16_gemm<128, 160, 4, 1, 1, 3, OUT>(p, st);
-  return launch_bf16_gemm<256, 160, 4, 1, 1, 3, OUT>(p, st);
+  const float a = tile_rounds(p, 64, 64) * 0.27f, b = tile_rounds(p, 128, 128) * 0.5f, c = tile_rounds(p, 128, 160) * 0.7f,
+              d = tile_rounds(p, 256, 160) * 1.1f;
+  if (a <= b && a <= c && a <= d) return launch_mx_gemm<64, 64, 1, 1, 4, 2, false, OUT>(p, st);
+  if (b <= c && b <= d) return launch_mx_gemm<128, 128, 2, 2, 1, 3, false, OUT>(p, st);
+  if (c <= d) return launch_mx_gemm<128, 160, 4, 1, 1, 3, false, OUT>(p, st);
+  return launch_mx_gemm<256, 160, 4, 1, 1, 3, false, OUT>(p, st);
 }
 
 }  // namespace ldm
@@ -804,6 +883,7 @@ extern "C" int ldm_mx4_linear(const void* x, const void* x_scale, const void* w,
                               int out_dtype, long long rows, int n, int k, void* stream) {
   LDM_REQUIRE(dtype_ok(out_dtype), "ldm_mx4_linear: bad dtype %d", out_dtype);
   LDM_REQUIRE(rows >= 0 && n >= 1 && k >= 1 && k <= (1 << 22), "ldm_mx4_linear: bad sizes (rows=%lld n=%d k=%d)", rows, n, k);
+  LDM_REQUIRE(rows < (1LL << 40) && ((rows + 63) / 64) * ((n + 63) / 64) < (1LL << 31), "ldm_mx4_linear: %lld x %d outputs are too many", rows, n);
   if (rows == 0) return LDM_OK;
   LDM_REQUIRE(x && w && w_scale && out, "ldm_mx4_linear: null pointer");
   const bool mx = x_scale != nullptr;
@@ -832,6 +912,7 @@ extern "C" int ldm_linear_bf16(const void* x, const void* w, const float* bias, 
   LDM_REQUIRE(dtype_ok(out_dtype), "ldm_linear_bf16: bad dtype %d", out_dtype);
   LDM_REQUIRE(rows >= 0 && n >= 1 && k >= 8 && k % 8 == 0 && k <= (1 << 21), "ldm_linear_bf16: bad sizes (rows=%lld n=%d k=%d; k a multiple of 8)",
               rows, n, k);
+  LDM_REQUIRE(rows < (1LL << 40) && ((rows + 63) / 64) * ((n + 63) / 64) < (1LL << 31), "ldm_linear_bf16: %lld x %d outputs are too many", rows, n);
   if (rows == 0) return LDM_OK;
   LDM_REQUIRE(x && w && out && aligned16(x) && aligned16(w) && (reinterpret_cast<uintptr_t>(bias) & 3) == 0 &&
                   reinterpret_cast<uintptr_t>(out) % dtype_size(out_dtype) == 0,
