@@ -112,6 +112,45 @@ def test_product_few_rows_wide_and_unaligned():
         assert mx.product_error(y, x[1:].view(6, 64).double(), mx_ref.quantize(w, 4)[2]) <= 0
 
 
+@pytest.mark.parametrize("dma", ["lazy", "eager"])
+@pytest.mark.parametrize("rows,n,k", [(66, 200, 2100), (130, 70, 777), (1100, 1300, 300), (1030, 1410, 1100), (2050, 4104, 200)])
+def test_product_both_4bit_tiles(rows, n, k, dma):
+    """Outputs of every tile's choice -- 64 x 64 with its columns split, 128 x 128, 256 x 256 -- with more steps than LDS has slots."""
+    with Guarded() as g, emulated(dma, guard=True) as ops:
+        mx.check_linear(ops, rows, n, k, 21, "mx4", bf if n % 4 else torch.float32, True, g.like)
+
+
+@pytest.mark.parametrize("dma", ["lazy", "eager"])
+@pytest.mark.parametrize("rows,n,k", [(66, 130, 1300), (70, 33, 8), (1030, 1000, 200), (500, 10230, 200), (1000, 10230, 200)])
+def test_product_bf16_tiles(rows, n, k, dma):
+    """Likewise for bfloat16 activations: 64 x 64, 128 x 128, 128 x 160, 256 x 160."""
+    with Guarded() as g, emulated(dma, guard=True) as ops:
+        mx.check_linear(ops, rows, n, k, 22, "bf16", bf if n % 3 else torch.float32, True, g.like)
+
+
+@pytest.mark.parametrize("act", ["mx4", "bf16"])
+@pytest.mark.parametrize("dma", ["lazy", "eager"])
+@pytest.mark.parametrize("rows,n,k", [(5, 24, 9000), (3, 20, 2049), (20, 18, 3100), (40, 18, 3100), (3, 4100, 300), (2, 12300, 70), (2, 16500, 64),
+                                      (20, 4100, 136), (40, 4100, 136)])
+def test_product_few_rows_variants(rows, n, k, dma, act):
+    """Fragments of the weights a workgroup from one to four, rings that wrap, an odd number of columns."""
+    with Guarded() as g, emulated(dma, guard=True) as ops:
+        mx.check_linear(ops, rows, n, k, 23, act, bf if n % 3 else torch.float32, True, g.like)
+
+
+@pytest.mark.parametrize("rows,n,k", [(3, 40, 160), (70, 72, 96), (70, 72, 160), (70, 72, 520), (70, 72, 1100), (1030, 1100, 520)])
+def test_product_nan_block_reaches_its_rows_only(rows, n, k):
+    """The last block of a row and the first of the next lie side by side, and so do their scales: a NaN in one of them stays there."""
+    x, w = seeded((rows, k), 1), seeded((n, k), 2)
+    x[1, k - 1], w[9, 0], w[20, k - 1] = math.nan, math.inf, math.nan
+    want = torch.zeros(rows, n, dtype=torch.bool)
+    want[1], want[:, 9], want[:, 20] = True, True, True
+    with Guarded() as g, emulated(guard=True) as ops:
+        wq = ops.mx4_quantize(g.like(w))
+        assert torch.equal(torch.isnan(ops.mx4_linear(ops.mx4_quantize(g.like(x)), wq)), want)
+        assert torch.equal(torch.isnan(ops.mx4_linear(g.like(x.to(bf)), wq)), want)
+
+
 @pytest.mark.parametrize("rows,n,k", [(70, 64, 96), (90, 50, 77)])
 def test_product_many_bf16_rows(rows, n, k):
     with Guarded() as g, emulated(guard=True) as ops:
@@ -258,6 +297,19 @@ def test_c_entries_refuse_without_a_launch():
     assert bad(lib.ldm_mx4_linear(p + 2, p, p, p, 0, p, 0, 1, 1, 1, 0))
     assert bad(lib.ldm_mx4_linear(p, p, p, p, 0, p, 0, 1, 1, (1 << 22) + 1, 0))
     assert lib.ldm_mx4_linear(0, 0, 0, 0, 0, 0, 0, 0, 1, 1, 0) == 0
+    assert bad(lib.ldm_mx4_linear(p, p, p, p, 0, p, 0, 1 << 39, 1 << 30, 1, 0))
+    assert bad(lib.ldm_linear_bf16(p, p, 0, p, 1, 1, 1, 12, 0))                               # k not a multiple of 8
+    assert bad(lib.ldm_linear_bf16(p + 2, p, 0, p, 1, 1, 1, 8, 0))
+    assert bad(lib.ldm_linear_bf16(p, p + 8, 0, p, 1, 1, 1, 8, 0))
+    assert bad(lib.ldm_linear_bf16(p, p, 0, p + 1, 1, 1, 1, 8, 0))
+    assert bad(lib.ldm_linear_bf16(p, p, 0, p, 5, 1, 1, 8, 0))
+    assert bad(lib.ldm_linear_bf16(p, p, 0, p, 1, 1 << 39, 1 << 30, 8, 0))
+    assert lib.ldm_linear_bf16(0, 0, 0, 0, 1, 0, 1, 8, 0) == 0
+    assert bad(lib.ldm_pad_columns_bf16(p, p, 1, 8, 12, 0))
+    assert bad(lib.ldm_pad_columns_bf16(p, p, 1, 9, 8, 0))
+    assert bad(lib.ldm_pad_columns_bf16(p + 1, p, 1, 7, 8, 0))
+    assert bad(lib.ldm_pad_columns_bf16(p, p + 2, 1, 7, 8, 0))
+    assert lib.ldm_pad_columns_bf16(0, 0, 0, 7, 8, 0) == 0
     assert bad(lib.ldm_linear_wgrad_mx8(p, p, p, p, 1, 12, 32, 0, 0, 0, 0))                   # n not a multiple of 8
     assert bad(lib.ldm_linear_wgrad_mx8(p, p, p, p, 0, 8, 32, 0, 0, 0, 0))
     need = lib.ldm_linear_wgrad_mx8_workspace_bytes(1 << 20, 8, 32)

@@ -83,6 +83,38 @@ def test_product_many_bf16_rows(rows, n, k):
     mx.check_linear(ops, rows, n, k, 15, "bf16", bf, True, dev)
 
 
+@pytest.mark.parametrize("rows,n,k", [(66, 200, 2100), (130, 70, 7777), (1100, 1300, 300), (1030, 1410, 4100), (2050, 4104, 2000)])
+def test_product_both_4bit_tiles(rows, n, k):
+    """Outputs of every tile's choice -- 64 x 64 with its columns split, 128 x 128, 256 x 256 -- with more steps than LDS has slots."""
+    mx.check_linear(ops, rows, n, k, 21, "mx4", bf if n % 4 else torch.float32, True, dev)
+
+
+@pytest.mark.parametrize("rows,n,k", [(66, 130, 1300), (70, 33, 8), (154, 1290, 5001), (1030, 1000, 2000), (500, 10230, 1000), (1000, 10230, 1000)])
+def test_product_bf16_tiles(rows, n, k):
+    """Likewise for bfloat16 activations: 64 x 64, 128 x 128, 128 x 160, 256 x 160."""
+    mx.check_linear(ops, rows, n, k, 22, "bf16", bf if n % 3 else torch.float32, True, dev)
+
+
+@pytest.mark.parametrize("act", ["mx4", "bf16"])
+@pytest.mark.parametrize("rows,n,k", [(5, 24, 9000), (3, 20, 2049), (20, 18, 3100), (40, 18, 3100), (3, 4100, 300), (2, 12300, 700), (2, 16500, 640),
+                                      (20, 4100, 1360), (40, 4100, 1360), (16, 10240, 4096)])
+def test_product_few_rows_variants(rows, n, k, act):
+    """Fragments of the weights a workgroup from one to four, rings that wrap, an odd number of columns."""
+    mx.check_linear(ops, rows, n, k, 23, act, bf if n % 3 else torch.float32, True, dev)
+
+
+@pytest.mark.parametrize("rows,n,k", [(3, 40, 160), (70, 72, 96), (70, 72, 160), (70, 72, 520), (70, 72, 1100), (1030, 1100, 520), (2050, 4104, 520)])
+def test_product_nan_block_of_a_neighbouring_row(rows, n, k):
+    """The last block of a row and the first of the next lie side by side, and so do their scales: a NaN in one of them stays there."""
+    x, w = seeded((rows, k), 1), seeded((n, k), 2)
+    x[1, k - 1], w[9, 0], w[20, k - 1] = math.nan, math.inf, math.nan
+    want = torch.zeros(rows, n, dtype=torch.bool)
+    want[1], want[:, 9], want[:, 20] = True, True, True
+    wq = ops.mx4_quantize(w.cuda())
+    assert torch.equal(torch.isnan(ops.mx4_linear(ops.mx4_quantize(x.cuda()), wq)).cpu(), want)
+    assert torch.equal(torch.isnan(ops.mx4_linear(x.to(bf).cuda(), wq)).cpu(), want)
+
+
 def test_product_leading_dimensions_and_unaligned_rows():
     w, x = seeded((40, 64), 5) / 8, seeded((1 + 6 * 64,), 6).to(bf)
     off = x.cuda()[1:].view(2, 3, 64)
@@ -107,6 +139,11 @@ def test_product_nan_block_reaches_its_rows_only():
 @pytest.mark.parametrize("rows,n,k", [(1, 32, 8), (70, 96, 64), (154, 1290, 765), (5, 200, 300), (1024, 5120, 640)])
 def test_input_gradient(rows, n, k):
     mx.check_dgrad(ops, rows, n, k, 17, dev)
+
+
+@pytest.mark.parametrize("rows,n,k", [(7, 4097, 96), (300, 2049, 640), (1030, 2560, 1000), (4100, 640, 1280)])
+def test_input_gradient_of_long_sums_and_odd_columns(rows, n, k):
+    mx.check_dgrad(ops, rows, n, k, 18, dev)
 
 
 def test_input_gradient_against_differences():
