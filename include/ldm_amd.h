@@ -431,8 +431,8 @@ int ldm_mx_quantize(const void* x, int dtype, long long rows, int cols, long lon
 int ldm_mx_dequantize(const void* data, const void* scale, int fmt, long long rows, int cols, void* out, int dtype, long long ld,
                       void* stream);
 
-/* The transposed values of LDM_MX4 rows in bfloat16: out[k][n], n = 0 .. rows-1, rows .. ld-1 zero (ld a multiple of 8): the filter
- * with which ldm_conv_gemm on dY computes the input gradient of a linear layer with 4-bit weights. */
+/* The transposed values of LDM_MX4 rows in bfloat16: out[k][n], n = 0 .. rows-1, rows .. ld-1 zero (ld a multiple of 8): the weights
+ * with which ldm_linear_bf16 on dY computes the input gradient of a linear layer with 4-bit weights. */
 int ldm_mx4_dequantize_t(const void* data, const void* scale, int rows, int cols, void* out, int ld, void* stream);
 
 /* GEGLU / SwiGLU whose backward pass reads an 8-bit checkpoint of the pre-activation (ldm_glu_forward / ldm_glu_backward keep it in the
@@ -448,7 +448,7 @@ int ldm_glu_backward_mx8(const void* data, const void* scale, const void* dout, 
 /* out (rows, n) = x W^T + bias (bias float32, may be NULL; out float32 or bfloat16, contiguous), W (n, k) in LDM_MX4.
  *   x_scale != NULL: x (rows, k) in LDM_MX4 as well: both operands go to the matrix cores as they are
  *   x_scale == NULL: x (rows, k) contiguous bfloat16 (any alignment); the weights are widened to bfloat16 (exact) in registers
- * Sums are float32.  Any rows >= 0, n >= 1, k >= 1.  x_scale == NULL reads W once for every 64 rows: meant for few rows. */
+ * Sums are float32.  Any rows >= 0, n >= 1, 1 <= k <= 2^22.  x_scale == NULL reads W once for every 64 rows: meant for few rows. */
 int ldm_mx4_linear(const void* x, const void* x_scale, const void* w, const void* w_scale, const float* bias, void* out, int out_dtype,
                    long long rows, int n, int k, void* stream);
 

@@ -1214,7 +1214,7 @@ def linear_wgrad_mx8(x8: MxTensor, dy: torch.Tensor, *, out: Optional[torch.Tens
     if rows == 0:
         return out if accumulate else out.zero_()
     npad = (n + 7) // 8 * 8
-    if npad != n:               # the kernel fetches dy in 16-byte pieces: odd widths go through a padded copy
+    if npad != n or dy.data_ptr() % 16:      # the kernel fetches dy in 16-byte pieces: other rows go through a padded copy
         full = linear_wgrad_mx8(x8, _pad_cols(dy.reshape(rows, n), npad).view(*dy.shape[:-1], npad))[:n]
         return out.add_(full) if accumulate else out.copy_(full)
     need = _lib.load().ldm_linear_wgrad_mx8_workspace_bytes(rows, n, k)

@@ -179,6 +179,15 @@ def test_weight_gradient(rows, n, k, acc, dma):
         mx.check_wgrad(ops, rows, n, k, 23, g.like, accumulate=acc)
 
 
+def test_gradients_of_rows_at_any_alignment():
+    x, flat = mx.activations(30, 72, 3), seeded((1 + 30 * 40,), 4).to(bf)
+    with Guarded() as g, emulated(guard=True) as ops:
+        off, dy = g.like(flat)[1:].view(30, 40), g.like(flat[1:].view(30, 40))
+        x8, w = ops.mx8_quantize(g.like(x)), ops.mx4_quantize(g.like(seeded((40, 72), 5)))
+        assert torch.equal(ops.linear_wgrad_mx8(x8, off), ops.linear_wgrad_mx8(x8, dy))
+        assert torch.equal(ops.mx4_linear_dgrad(off, w), ops.mx4_linear_dgrad(dy, w))
+
+
 def test_weight_gradient_of_nan_blocks_stays_in_their_columns():
     x = seeded((40, 96), 1)
     x[7, 40] = math.nan

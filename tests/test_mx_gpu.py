@@ -191,6 +191,21 @@ def test_weight_gradient(rows, n, k, acc):
     mx.check_wgrad(ops, rows, n, k, 23, dev, accumulate=acc)
 
 
+def test_gradients_of_rows_at_any_alignment():
+    x, flat = mx.activations(100, 72, 3), seeded((1 + 100 * 40,), 4).to(bf)
+    off, dy = flat.cuda()[1:].view(100, 40), flat[1:].view(100, 40)
+    assert off.data_ptr() % 16
+    x8, w = ops.mx8_quantize(x.cuda()), ops.mx4_quantize(seeded((40, 72), 5).cuda())
+    assert same_bits(ops.linear_wgrad_mx8(x8, off), ops.linear_wgrad_mx8(x8, dy.cuda()))
+    first = seeded((40, 72), 6).cuda()
+    a, b = first.clone(), first.clone()
+    ops.linear_wgrad_mx8(x8, off, out=a)
+    ops.linear_wgrad_mx8(x8, dy.cuda(), out=b)
+    # sums of both take the first values in at another place: half a float32 step of it and of the sum each
+    assert float((a - b).abs().max()) <= 2.0 ** -23 * float(b.abs().max() + first.abs().max())
+    assert same_bits(ops.mx4_linear_dgrad(off, w), ops.mx4_linear_dgrad(dy.cuda(), w))
+
+
 def test_repeated_calls_give_the_same_bits():
     x, dy = mx.activations(4096, 320, 1).cuda(), seeded((4096, 640), 2).to(bf).cuda()
     w = ops.mx4_quantize(seeded((640, 320), 3).cuda())
