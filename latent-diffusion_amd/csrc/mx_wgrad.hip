@@ -21,6 +21,7 @@ namespace ldm {
 typedef __attribute__((ext_vector_type(8))) short bf16x8_t;
 typedef __attribute__((ext_vector_type(4))) short bf16x4_t;
 typedef __attribute__((ext_vector_type(4))) float f32x4_t;
+typedef __attribute__((ext_vector_type(4))) int i32x4_t;
 
 struct WgradMx8Params {
   const unsigned char* x;
@@ -57,7 +58,24 @@ __device__ __forceinline__ void wm8_dma4(const void* base, int bytes, unsigned c
   const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, 0x00020000);
   __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)lds, 4, voff, 0, 0, 0);
 }
-// transposed LDS read; the caller waits before it uses the value
+// LDS accesses in assembly; the caller waits before it uses what it reads.  In front of reads and writes of its own the compiler waits for
+// every LDS-DMA in flight -- here for the next step's, which had just been issued: 86 us instead of WGRAD_US at 32768 x 2560 x 320.
+template <int OFF>
+__device__ __forceinline__ void lds_read16(i32x4_t& v, unsigned addr) {
+  asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(v) : "v"(addr), "n"(OFF) : "memory");
+}
+template <int OFF>
+__device__ __forceinline__ void lds_read4(int& v, unsigned addr) {
+  asm volatile("ds_read_b32 %0, %1 offset:%2" : "=v"(v) : "v"(addr), "n"(OFF) : "memory");
+}
+template <int OFF>
+__device__ __forceinline__ void lds_write16(unsigned addr, i32x4_t v) {
+  asm volatile("ds_write_b128 %0, %1 offset:%2" ::"v"(addr), "v"(v), "n"(OFF) : "memory");
+}
+// no use of v moves above the wait in front of this
+__device__ __forceinline__ void stay_below(i32x4_t& v) { asm volatile("" : "+v"(v)); }
+__device__ __forceinline__ void stay_below(int& v) { asm volatile("" : "+v"(v)); }
+// transposed
 template <int OFF>
 __device__ __forceinline__ void tr_read(bf16x4_t& v, unsigned addr) {
   asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2" : "=v"(v) : "v"(addr), "n"(OFF) : "memory");
@@ -171,29 +189,35 @@ linear_wgrad_mx8_kernel(const WgradMx8Params p) {
     udst[u] = IMG0 + row * (T1 * 2) + (((2 * half) ^ wm8_swz<T1>(row)) << 4);
     ubyte[u] = 8 * (((k0 >> 5) + (half >> 1)) & 3);
   }
-  uint4 xraw[UMAX];
-  unsigned xcode[UMAX];
+  const unsigned lds_base = (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
+  i32x4_t xraw[UMAX];
+  int xcode[UMAX];
   auto read_raw = [&](int place) {
 #pragma unroll
     for (int u = 0; u < UMAX; ++u) {
-      xraw[u] = make_uint4(0, 0, 0, 0);
+      xraw[u] = i32x4_t{0, 0, 0, 0};
       xcode[u] = 0;
       if (has_unit(u)) {
-        xraw[u] = *reinterpret_cast<const uint4*>(raw + place * RAW + (u * 512 + tid) * 16);
-        xcode[u] = *reinterpret_cast<const unsigned*>(raw + place * RAW + UNITS * 16 + (u * 512 + tid) * 4);
+        lds_read16<0>(xraw[u], lds_base + 2 * SLOT + place * RAW + (u * 512 + tid) * 16);
+        lds_read4<UNITS * 16>(xcode[u], lds_base + 2 * SLOT + place * RAW + (u * 512 + tid) * 4);
       }
     }
+  };
+  auto raw_here = [&] {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int u = 0; u < UMAX; ++u) { stay_below(xraw[u]); stay_below(xcode[u]); }
   };
   uint32_t wide[8];
   float one = 0.f;
   auto widen_begin = [&](auto unit) {
     constexpr int u = decltype(unit)::value;
-    const int code = (int)(xcode[u] >> ubyte[u]) & 255;
+    const int code = (xcode[u] >> ubyte[u]) & 255;
     one = code == 255 ? __uint_as_float(0x7fc00000u) : ldexpf(1.0f, code - 133);
   };
   auto widen_word = [&](auto unit, auto word) {            // four elements
     constexpr int u = decltype(unit)::value, i = decltype(word)::value;
-    const unsigned w = i == 0 ? xraw[u].x : i == 1 ? xraw[u].y : i == 2 ? xraw[u].z : xraw[u].w;
+    const unsigned w = (unsigned)xraw[u][i];
     float v[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = (float)((int)(w << (24 - 8 * e)) >> 24) * one;
@@ -206,10 +230,10 @@ linear_wgrad_mx8_kernel(const WgradMx8Params p) {
   };
   auto write_wide = [&](auto unit, int slot) {
     constexpr int u = decltype(unit)::value;
-    uint4* d = reinterpret_cast<uint4*>(smem + slot * SLOT + udst[u]);
     if (has_unit(u)) {
-      d[0] = make_uint4(wide[0], wide[1], wide[2], wide[3]);
-      d[1] = make_uint4(wide[4], wide[5], wide[6], wide[7]);
+      const unsigned d = lds_base + slot * SLOT + udst[u];
+      lds_write16<0>(d, i32x4_t{(int)wide[0], (int)wide[1], (int)wide[2], (int)wide[3]});
+      lds_write16<16>(d, i32x4_t{(int)wide[4], (int)wide[5], (int)wide[6], (int)wide[7]});
     }
   };
   using First = std::integral_constant<int, 0>;
@@ -225,7 +249,6 @@ linear_wgrad_mx8_kernel(const WgradMx8Params p) {
   // half tp & 1
   const int fr = lane & 15, fq = lane >> 4, tq = fr >> 2, tp = fr & 3;
   const int frow = 4 * fq + tq;
-  const unsigned lds_base = (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
   constexpr int NO0 = wm8_distinct<T0, F0>(), NO1 = wm8_distinct<T1, F1>();
   unsigned off0[NO0], off1[NO1];
 #pragma unroll
@@ -292,6 +315,7 @@ linear_wgrad_mx8_kernel(const WgradMx8Params p) {
     if (nsteps > 1) load_x(1);
     arrive();
     read_raw(0);
+    raw_here();
     widen(First{});
     write_wide(First{}, 0);
     if constexpr (UMAX > 1) { widen(Last{}); write_wide(Last{}, 0); }
@@ -303,8 +327,7 @@ linear_wgrad_mx8_kernel(const WgradMx8Params p) {
     };
     for (int s = 0; s < nsteps; ++s) {
       // Behind the barrier dY(s) and the widened x(s) are in slot s & 1, the stored x(s + 1) is in place (s + 1) & 1, and nobody reads
-      // slot (s + 1) & 1 or place s & 1 any more.  The plain LDS reads come before the first load: the compiler drains a wave's loads in
-      // front of one.
+      // slot (s + 1) & 1 or place s & 1 any more.
       arrive();
       const int cur = s & 1, next = cur ^ 1;
       const bool more = s + 1 < nsteps;
@@ -318,6 +341,7 @@ linear_wgrad_mx8_kernel(const WgradMx8Params p) {
         end_dy();
       }
       if (s + 2 < nsteps) load_x(cur);
+      raw_here();
       // waves 0 .. 3 widen the next x behind their MFMAs, waves 4 .. 7 -- the other wave of each SIMD -- in front of them, so that a SIMD's
       // matrix core works for one while the other converts
       if (wave >= 4 && more) next_x(next);

@@ -9,7 +9,7 @@ The sources are compiled as they are, after a textual pass over the constructs t
   * ``asm volatile("s_waitcnt lgkmcnt ...")``  -> a wave rendezvous (lanes exchange data through LDS around it)
   * empty asm fences / register pins           -> dropped
   * ``asm volatile("ds_read_b64_tr_b16 ...")`` -> the emulated transposed read
-  * ``asm volatile("ds_read_b128 / _b32 ...")`` -> a plain read at the LDS address
+  * ``asm volatile("ds_read_b128 / _b32 ...")``, ``ds_write_b128`` -> a plain access at the LDS address
 The transformed copies live only under _build/ (git-ignored)."""
 import hashlib
 import os
@@ -94,6 +94,8 @@ def _asm_replacement(body, where):
     m = re.fullmatch(r"ds_read_b(32|128) %0, %1 offset:%2", t)
     if m:
         return f"::emu::ds_read_lds_addr<{int(m.group(1)) // 8}>({outs[0]}, {ins[0]}, {ins[1]})"
+    if re.fullmatch(r"ds_write_b128 %0, %1 offset:%2", t):
+        return f"::emu::ds_write_lds_addr<16>({ins[0]}, {ins[1]}, {ins[2]})"
     raise ValueError(f"{where}: inline asm not understood: {t!r}")
 
 

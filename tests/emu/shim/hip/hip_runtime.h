@@ -171,6 +171,13 @@ static inline void ds_read_lds_addr(V& out, unsigned lds_addr, int off) {
   if (rel % BYTES) { fprintf(stderr, "emu: ds_read_b%d at LDS address %u\n", 8 * BYTES, rel); abort(); }
   memcpy(&out, dyn_smem() + rel, BYTES);
 }
+template <int BYTES, class V>
+static inline void ds_write_lds_addr(unsigned lds_addr, const V& v, int off) {
+  static_assert(sizeof(V) == BYTES, "ds_write data");
+  const unsigned rel = lds_addr + (unsigned)off - (unsigned)(uintptr_t)dyn_smem();
+  if (rel % BYTES) { fprintf(stderr, "emu: ds_write_b%d at LDS address %u\n", 8 * BYTES, rel); abort(); }
+  memcpy(dyn_smem() + rel, &v, BYTES);
+}
 EMU_NOINLINE inline void wave_barrier() { wave_op(OP_WAVE_BARRIER, __builtin_return_address(0), nullptr, nullptr); }
 
 // buffer resources: base + byte count; an access whose last byte lies past the count returns zeros
