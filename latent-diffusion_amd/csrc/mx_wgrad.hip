@@ -7,10 +7,15 @@
 // of what the bf16 activation would.
 //
 // The contraction runs over the rows of both operands.  A workgroup of 8 waves owns T0 columns of dY x T1 columns of x and walks its
-// share of the rows 64 a step, double-buffered: dY goes to LDS by LDS-DMA one step ahead; x goes there by LDS-DMA two steps ahead as it
-// is stored, and the thread that fetched 16 of its elements widens them into the bf16 image one step ahead.  Both operands' fragments
-// are read transposed (ds_read_b64_tr_b16, the same permutation of the rows on both sides).  The rows are split over blockIdx.y where
-// there are few tiles; the partial tiles are added by a second kernel in a fixed order (no atomics).
+// share of the rows 64 a step, double-buffered: dY goes to LDS by LDS-DMA; x goes there by LDS-DMA as it is stored, and the thread that
+// fetched 16 of its elements widens them into the bf16 image one step ahead.  Both operands' fragments are read transposed
+// (ds_read_b64_tr_b16, the same permutation of the rows on both sides), each block of 32 rows while the block before multiplies.  The
+// rows are split over workgroups where there are few tiles; the partial tiles are added by a second kernel in a fixed order (no
+// atomics).
+//
+// 32768 rows, 2560 x 320 (54 GFLOP, 180 MB): 70 us + 12 us for the 16 partial tiles, 650 TFLOP/s; a large bf16 matrix product reaches
+// 1170.  What is left between: LDS (the transposed reads of a step take 0.8 of its matrix time, dY's arrival and the widened
+// image 0.4 more), and 52 MB of partial tiles written and read.
 #include "common.h"
 
 #include <type_traits>
@@ -59,7 +64,7 @@ __device__ __forceinline__ void wm8_dma4(const void* base, int bytes, unsigned c
   __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)lds, 4, voff, 0, 0, 0);
 }
 // LDS accesses in assembly; the caller waits before it uses what it reads.  In front of reads and writes of its own the compiler waits for
-// every LDS-DMA in flight -- here for the next step's, which had just been issued: 86 us instead of WGRAD_US at 32768 x 2560 x 320.
+// every LDS-DMA in flight -- here for the next step's, which had just been issued: 86 us instead of 76 at 32768 x 2560 x 320.
 template <int OFF>
 __device__ __forceinline__ void lds_read16(i32x4_t& v, unsigned addr) {
   asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(v) : "v"(addr), "n"(OFF) : "memory");
@@ -139,6 +144,7 @@ linear_wgrad_mx8_kernel(const WgradMx8Params p) {
   }
   const int dy_row = p.n * 2, xd_row = p.blocks * 32;
   auto rows_of = [&](int step) {                           // rows of a step inside the matrix
+    if (step >= step_begin + nsteps) return 0;             // fetched like any other: zeros that nobody reads
     return step == total_steps - 1 ? (int)(p.rows - (long long)step * WM8_MS) : WM8_MS;
   };
   // the loads of the step being issued: set up once a step, then issued one instruction at a time between MFMAs
@@ -259,23 +265,17 @@ linear_wgrad_mx8_kernel(const WgradMx8Params p) {
     off1[j] = lds_base + IMG0 + frow * (T1 * 2) + (((2 * (w1 * F1 + j) + (tp >> 1)) ^ wm8_swz<T1>(frow)) << 4) + ((tp & 1) << 3);
 
   struct Frags { bf16x4_t lo0[F0], hi0[F0], lo1[F1], hi1[F1]; };
-  auto read_fragments = [&](Frags& f, int slot, auto block) {
-    constexpr int B = decltype(block)::value;
-    const unsigned sbase = slot * SLOT;
-    [&]<int... I>(std::integer_sequence<int, I...>) {
-      ([&] {
-        constexpr int i = I;
-        tr_read<i / NO0 * (NO0 * 32) + B * 32 * T0 * 2>(f.lo0[i], sbase + off0[i % NO0]);
-        tr_read<i / NO0 * (NO0 * 32) + (B * 32 + 16) * T0 * 2>(f.hi0[i], sbase + off0[i % NO0]);
-      }(), ...);
-    }(std::make_integer_sequence<int, F0>{});
-    [&]<int... J>(std::integer_sequence<int, J...>) {
-      ([&] {
-        constexpr int j = J;
-        tr_read<j / NO1 * (NO1 * 32) + B * 32 * T1 * 2>(f.lo1[j], sbase + off1[j % NO1]);
-        tr_read<j / NO1 * (NO1 * 32) + (B * 32 + 16) * T1 * 2>(f.hi1[j], sbase + off1[j % NO1]);
-      }(), ...);
-    }(std::make_integer_sequence<int, F1>{});
+  // fragment Q (dY's, then x's) of 32-row block B of a slot
+  auto read_fragment = [&]<int B, int Q>(std::integral_constant<int, B>, std::integral_constant<int, Q>, Frags& f, unsigned sbase) {
+    if constexpr (Q < F0) {
+      constexpr int i = Q;
+      tr_read<i / NO0 * (NO0 * 32) + B * 32 * T0 * 2>(f.lo0[i], sbase + off0[i % NO0]);
+      tr_read<i / NO0 * (NO0 * 32) + (B * 32 + 16) * T0 * 2>(f.hi0[i], sbase + off0[i % NO0]);
+    } else {
+      constexpr int j = Q - F0;
+      tr_read<j / NO1 * (NO1 * 32) + B * 32 * T1 * 2>(f.lo1[j], sbase + off1[j % NO1]);
+      tr_read<j / NO1 * (NO1 * 32) + (B * 32 + 16) * T1 * 2>(f.hi1[j], sbase + off1[j % NO1]);
+    }
   };
   auto here = [&](Frags& f) {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -284,20 +284,29 @@ linear_wgrad_mx8_kernel(const WgradMx8Params p) {
 #pragma unroll
     for (int j = 0; j < F1; ++j) asm volatile("" : "+v"(f.lo1[j]), "+v"(f.hi1[j]));
   };
-  auto multiply = [&](const Frags& f) {
+  // a block's products; behind the first of them the reads of block B into `ahead`, behind the others -- with DY -- dY's loads
+  auto multiply = [&]<int B, bool DY>(const Frags& f, Frags& ahead, unsigned sbase, std::integral_constant<int, B> block, std::integral_constant<bool, DY>) {
     auto join = [](const bf16x4_t& lo, const bf16x4_t& hi) {
       return bf16x8_t{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     };
     __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-    for (int i = 0; i < F0; ++i)
-#pragma unroll
-      for (int j = 0; j < F1; ++j)
+    [&]<int... Q>(std::integer_sequence<int, Q...>) {
+      ([&] {
+        constexpr int q = Q, i = q / F1, j = q % F1, FF = F0 + F1, MM = F0 * F1;
         acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(join(f.lo1[j], f.hi1[j]), join(f.lo0[i], f.hi0[i]), acc[i][j], 0, 0, 0);
-    __builtin_amdgcn_s_setprio(0);
-    __builtin_amdgcn_sched_barrier(0);
+        if constexpr (q < FF) read_fragment(block, std::integral_constant<int, q>{}, ahead, sbase);
+        if constexpr (DY) {
+#pragma unroll
+          for (int d = q * ND / MM; d < (q + 1) * ND / MM; ++d) issue_dy(d);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }(), ...);
+    }(std::make_integer_sequence<int, F0 * F1>{});
   };
+  static_assert(F0 + F1 <= F0 * F1, "a read behind each product");
+  constexpr std::integral_constant<int, 0> B0{};
+  constexpr std::integral_constant<int, 1> B1{};
+
   if (nsteps > 0) {
     auto arrive = [&]() {                                  // what this wave loaded and wrote is there, and then everybody's is
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -307,52 +316,54 @@ linear_wgrad_mx8_kernel(const WgradMx8Params p) {
       asm volatile("" ::: "memory");
       __builtin_amdgcn_sched_barrier(0);
     };
-    load_x(0);
-    begin_dy(0);
+    auto load_dy = [&](int slot) {
+      begin_dy(slot);
 #pragma unroll
-    for (int j = 0; j < ND; ++j) issue_dy(j);
-    end_dy();
-    if (nsteps > 1) load_x(1);
-    arrive();
-    read_raw(0);
-    raw_here();
-    widen(First{});
-    write_wide(First{}, 0);
-    if constexpr (UMAX > 1) { widen(Last{}); write_wide(Last{}, 0); }
-    Frags f;
+      for (int j = 0; j < ND; ++j) issue_dy(j);
+      end_dy();
+    };
     auto next_x = [&](int slot) {
       widen(First{});
       write_wide(First{}, slot);
       if constexpr (UMAX > 1) { widen(Last{}); write_wide(Last{}, slot); }
     };
+    Frags f0, f1;
+    load_x(0);
+    load_dy(0);
+    load_x(1);
+    arrive();
+    read_raw(0);
+    raw_here();
+    next_x(0);
+    load_dy(1);
+    load_x(0);
+    arrive();
+    read_raw(1);
+    [&]<int... Q>(std::integer_sequence<int, Q...>) {
+      (read_fragment(B0, std::integral_constant<int, Q>{}, f0, 0u), ...);
+    }(std::make_integer_sequence<int, F0 + F1>{});
+    here(f0);
+    raw_here();
+    // At the top of step s: block 0 of slot s & 1 in f0, the stored x(s + 1) in registers, x(s + 2) in place s & 1, dY(s + 1) in or on its way to
+    // the other slot.  The barrier in the middle frees the step's slot (its block 1 is in registers) and says that the next one is
+    // whole; x(s + 1) is widened in front of block 0 by waves 4 .. 7 and behind it by waves 0 .. 3 -- the other wave of each SIMD -- so
+    // that the SIMD's matrix core works for one while the other converts.
     for (int s = 0; s < nsteps; ++s) {
-      // Behind the barrier dY(s) and the widened x(s) are in slot s & 1, the stored x(s + 1) is in place (s + 1) & 1, and nobody reads
-      // slot (s + 1) & 1 or place s & 1 any more.
-      arrive();
       const int cur = s & 1, next = cur ^ 1;
-      const bool more = s + 1 < nsteps;
-      read_raw(next);
-      asm volatile("" ::: "memory");
-      __builtin_amdgcn_sched_barrier(0);
-      if (more) {
-        begin_dy(next);
-#pragma unroll
-        for (int j = 0; j < ND; ++j) issue_dy(j);
-        end_dy();
-      }
-      if (s + 2 < nsteps) load_x(cur);
+      if (wave >= 4) next_x(next);
+      multiply(f0, f1, (unsigned)cur * SLOT, B1, std::false_type{});
+      if (wave < 4) next_x(next);
+      here(f1);
+      arrive();
+      read_raw(cur);
+      begin_dy(cur);
+      load_x(next);
+      multiply(f1, f0, (unsigned)next * SLOT, B0, std::true_type{});
+      end_dy();
+      here(f0);
       raw_here();
-      // waves 0 .. 3 widen the next x behind their MFMAs, waves 4 .. 7 -- the other wave of each SIMD -- in front of them, so that a SIMD's
-      // matrix core works for one while the other converts
-      if (wave >= 4 && more) next_x(next);
-      read_fragments(f, cur, std::integral_constant<int, 0>{});
-      here(f);
-      multiply(f);
-      read_fragments(f, cur, std::integral_constant<int, 1>{});
-      here(f);
-      multiply(f);
-      if (wave < 4 && more) next_x(next);
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   }
 
   // x is the instruction's first operand: a lane has four consecutive k (rows 4 fq .. + 3 of the fragment) of one n (column fr)

@@ -40,23 +40,47 @@ def _registers(text):
 
 
 def pending_read_hazards(listing):
-    """(LDS reads seen, instructions that touch a destination of one before a wait for it), in program order."""
-    reads, bad, pending = 0, [], []
+    """(LDS reads seen, instructions that touch a destination of one before a wait for it), along every path through the listing.
+    What is carried along: for each register that a read will fill, how many LDS operations have been issued since on the path with the
+    fewest (lgkmcnt(n) waits for all that n or more others followed)."""
+    code = []
     for line in listing.splitlines():
-        ins = line.split("//")[0].strip()
-        if ins.startswith("s_waitcnt"):
-            m = re.search(r"lgkmcnt\((\d+)\)", ins)
-            if m:
-                pending = pending[len(pending) - int(m.group(1)):] if len(pending) > int(m.group(1)) > 0 else (pending if int(m.group(1)) else [])
+        ins, _, where = line.partition("//")
+        if ins.strip():
+            op, _, rest = ins.strip().partition(" ")
+            code.append((op, rest.strip(), int(where.split(":")[0], 16) if where.strip() else len(code), _registers(rest)))
+    at = {addr: i for i, (_, _, addr, _) in enumerate(code)}
+    state, bad, work = {0: {}}, set(), [0]
+
+    def reach(i, pending):
+        old = state.get(i)
+        new = dict(pending) if old is None else {r: min(old.get(r, 99), pending.get(r, 99)) for r in {*old, *pending}}
+        if new != old:
+            state[i] = new
+            work.append(i)
+
+    while work:
+        i = work.pop()
+        if i >= len(code):
             continue
-        if pending and _registers(ins) & set().union(*pending):
-            bad.append(ins)
-        if ins.startswith("ds_read"):
-            pending.append(_registers(ins.split(None, 1)[1].split(",")[0]))
-            reads += 1
-        elif ins.startswith("ds_"):
-            pending.append(set())
-    return reads, bad
+        pending = dict(state[i])
+        op, rest, addr, regs = code[i]
+        if op == "s_waitcnt":
+            m = re.search(r"lgkmcnt\((\d+)\)", rest)
+            if m:
+                pending = {r: n for r, n in pending.items() if n < int(m.group(1))}
+        elif regs & pending.keys():
+            bad.add(f"{op} {rest}")
+        if op.startswith("ds_"):
+            pending = {r: min(n + 1, 64) for r, n in pending.items()}
+            if op.startswith("ds_read"):
+                pending.update(dict.fromkeys(_registers(rest.split(",")[0]), 0))
+        if op == "s_branch" or op.startswith("s_cbranch"):
+            step = int(rest.split()[0])
+            reach(at[addr + 4 + 4 * (step - 65536 if step > 32767 else step)], pending)
+        if op not in ("s_branch", "s_endpgm"):
+            reach(i + 1, pending)
+    return sum(op.startswith("ds_read") for op, _, _, _ in code), sorted(bad)
 
 
 def test_the_hazard_check_finds_one():
@@ -64,6 +88,9 @@ def test_the_hazard_check_finds_one():
     assert pending_read_hazards(good) == (1, [])
     early = "ds_read_b128 v[4:7], v1\nds_read_b32 v9, v1\ns_waitcnt lgkmcnt(1)\nv_mov_b32 v2, v7\nv_mov_b32 v3, v9\n"
     assert pending_read_hazards(early) == (2, ["v_mov_b32 v3, v9"])
+    # around a loop: the read at its end is under way when the body begins again; the code behind the branch is not on the way
+    loop = ("s_nop 0 // 00: x\nv_mov_b32 v2, v9 // 04: x\nds_read_b32 v9, v1 // 08: x\ns_branch 65533 // 0c: x\nv_mov_b32 v3, v9 // 10: x\n")
+    assert pending_read_hazards(loop) == (1, ["ds_read_b32 v9, v1", "v_mov_b32 v2, v9"])
 
 
 @pytest.mark.parametrize("name", ["mx_gemm.hip.o", "mx_wgrad.hip.o"])
