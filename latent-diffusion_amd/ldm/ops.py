@@ -1204,19 +1204,17 @@ def linear_wgrad_mx8(x8: MxTensor, dy: torch.Tensor, *, out: Optional[torch.Tens
         raise ValueError(f"linear_wgrad_mx8: dy must be a contiguous {(*x8.shape[:-1], 'n')} tensor, got {tuple(dy.shape)}")
     _same_device("linear_wgrad_mx8", dy, x8.data, out)
     n, k, rows = dy.shape[-1], x8.cols, x8.rows
-    if accumulate is None:
-        accumulate = out is not None
-    if out is None:
-        accumulate = False
-        out = torch.empty((n, k), dtype=torch.float32, device=dy.device)
-    elif out.dtype != torch.float32 or tuple(out.shape) != (n, k) or not out.is_contiguous():
+    if out is not None and (out.dtype != torch.float32 or tuple(out.shape) != (n, k) or not out.is_contiguous()):
         raise ValueError(f"linear_wgrad_mx8: out must be a contiguous float32 tensor of shape {(n, k)}")
+    accumulate = out is not None and (accumulate is None or bool(accumulate))
+    npad = (n + 7) // 8 * 8
+    if rows and (npad != n or dy.data_ptr() % 16):      # the kernel fetches dy in 16-byte pieces: other rows go through a padded copy
+        full = linear_wgrad_mx8(x8, _pad_cols(dy.reshape(rows, n), npad).view(*dy.shape[:-1], npad))[:n]
+        return full if out is None else out.add_(full) if accumulate else out.copy_(full)
+    if out is None:
+        out = torch.empty((n, k), dtype=torch.float32, device=dy.device)
     if rows == 0:
         return out if accumulate else out.zero_()
-    npad = (n + 7) // 8 * 8
-    if npad != n or dy.data_ptr() % 16:      # the kernel fetches dy in 16-byte pieces: other rows go through a padded copy
-        full = linear_wgrad_mx8(x8, _pad_cols(dy.reshape(rows, n), npad).view(*dy.shape[:-1], npad))[:n]
-        return out.add_(full) if accumulate else out.copy_(full)
     need = _lib.load().ldm_linear_wgrad_mx8_workspace_bytes(rows, n, k)
     # from the allocator, not kept: a graph that captured the call owns its own, and no other call or graph writes to it
     ws = torch.empty(need, dtype=torch.uint8, device=dy.device) if need else None
