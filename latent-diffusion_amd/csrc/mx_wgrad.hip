@@ -378,13 +378,21 @@ linear_wgrad_mx8_kernel(const WgradMx8Params p) {
   }
 }
 
-// dw (+)= the partial tiles, in order
+// dw (+)= the partial tiles, in order.  The loads of eight are under way at a time: one by one they would wait for each other.
 __global__ void __launch_bounds__(256)
 wgrad_mx8_fold_kernel(const float* __restrict__ partial, float* __restrict__ dw, long long total, int splits, int accumulate) {
   const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
   if (i >= total) return;
   float v = accumulate ? dw[i] : 0.f;
-  for (int s = 0; s < splits; ++s) v += partial[(long long)s * total + i];
+  int s = 0;
+  for (; s + 8 <= splits; s += 8) {
+    float o[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] = partial[(long long)(s + j) * total + i];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v += o[j];
+  }
+  for (; s < splits; ++s) v += partial[(long long)s * total + i];
   dw[i] = v;
 }
 

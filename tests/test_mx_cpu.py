@@ -179,6 +179,12 @@ def test_weight_gradient(rows, n, k, acc, dma):
         mx.check_wgrad(ops, rows, n, k, 23, g.like, accumulate=acc)
 
 
+@pytest.mark.parametrize("rows", [700, 2900])
+def test_weight_gradient_of_many_splits(rows):
+    with Guarded() as g, emulated(guard=True) as ops:
+        mx.check_wgrad(ops, rows, 24, 40, 24, g.like, accumulate=rows == 2900)
+
+
 def test_gradients_of_rows_at_any_alignment():
     x, flat = mx.activations(30, 72, 3), seeded((1 + 30 * 40,), 4).to(bf)
     with Guarded() as g, emulated(guard=True) as ops:

@@ -191,6 +191,12 @@ def test_weight_gradient(rows, n, k, acc):
     mx.check_wgrad(ops, rows, n, k, 23, dev, accumulate=acc)
 
 
+@pytest.mark.parametrize("rows", [700, 2900, 5200])
+def test_weight_gradient_of_many_splits(rows):
+    """Two, eleven and twenty ranges of rows, added up by the second kernel."""
+    mx.check_wgrad(ops, rows, 24, 40, 24, dev, accumulate=rows == 2900)
+
+
 def test_gradients_of_rows_at_any_alignment():
     x, flat = mx.activations(100, 72, 3), seeded((1 + 100 * 40,), 4).to(bf)
     off, dy = flat.cuda()[1:].view(100, 40), flat[1:].view(100, 40)
