@@ -995,13 +995,14 @@ class MxTensor:
 
 
 def _same_device(what: str, ref: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
+    index = ref.get_device()
     for t in others:
-        if t is not None and t.device != ref.device:
+        if t is not None and t.get_device() != index:
             raise ValueError(f"{what}: operands on {ref.device} and {t.device}")
 
 
 def _mx(what: str, q, fmt: int) -> None:
-    if not isinstance(q, MxTensor) or q.fmt != fmt:
+    if not isinstance(q, MxTensor) or q.data.dtype != (torch.uint8 if fmt == _lib.MX4 else torch.int8):
         raise TypeError(f"{what} must be an MxTensor with {'4' if fmt == _lib.MX4 else '8'}-bit elements")
     _gpu(q.data, q.scale)
 
@@ -1009,8 +1010,10 @@ def _mx(what: str, q, fmt: int) -> None:
 def _mx_empty(lead, cols: int, fmt: int, device) -> MxTensor:
     blocks = (cols + 31) // 32
     q = MxTensor.__new__(MxTensor)          # laid out here: nothing for the constructor to check
-    q.data = torch.empty((*lead, blocks * (16 if fmt == _lib.MX4 else 32)), dtype=torch.uint8 if fmt == _lib.MX4 else torch.int8,
-                         device=device)
+    if fmt == _lib.MX4:
+        q.data = torch.empty((*lead, blocks * 16), dtype=torch.uint8, device=device)
+    else:
+        q.data = torch.empty((*lead, blocks * 32), dtype=torch.int8, device=device)
     q.scale = torch.empty((*lead, (blocks + 3) // 4 * 4), dtype=torch.uint8, device=device)
     q.cols = cols
     return q
@@ -1061,8 +1064,8 @@ def mx_dequantize(q: MxTensor, dtype: torch.dtype) -> torch.Tensor:
     if not isinstance(q, MxTensor):
         raise TypeError("mx_dequantize: an MxTensor expected")
     _gpu(q.data, q.scale)
-    out = torch.empty(q.shape, dtype=dtype, device=q.data.device)
     code = dt_code(dtype)
+    out = torch.empty((*q.data.shape[:-1], q.cols), dtype=dtype, device=q.data.device)
     if out.numel():
         _call(out, "ldm_mx_dequantize", q.data.data_ptr(), q.scale.data_ptr(), q.fmt, q.rows, q.cols, out.data_ptr(), code, q.cols)
     return out
@@ -1096,25 +1099,27 @@ def mx4_linear(x, w: MxTensor, bias: Optional[torch.Tensor] = None, out_dtype: O
     _mx("mx4_linear: w", w, _lib.MX4)
     if w.data.dim() != 2:
         raise ValueError(f"mx4_linear: w must be (n, k), got {tuple(w.shape)}")
-    n, k = w.shape
+    n, k = w.data.shape[0], w.cols
     mx = isinstance(x, MxTensor)
     if mx:
         _mx("mx4_linear: x", x, _lib.MX4)
+        xt, xk = x.data, x.cols
     else:
         _gpu(x)
         if x.dtype != torch.bfloat16:
             raise TypeError(f"mx4_linear: x must be bfloat16 or an MxTensor (got {x.dtype})")
         if not x.is_contiguous():
             raise ValueError("mx4_linear: x must be contiguous")
-    if len(x.shape) < 1 or x.shape[-1] != k:
+        xt, xk = x, x.shape[-1] if x.dim() else 0
+    if xk != k:
         raise ValueError(f"mx4_linear: x {tuple(x.shape)} does not match w {tuple(w.shape)}")
     odt = out_dtype or torch.bfloat16
     code = dt_code(odt)
-    _gpu(bias)
-    _f32_dense("mx4_linear: bias", bias, n)
-    xt = x.data if mx else x
+    if bias is not None:
+        _gpu(bias)
+        _f32_dense("mx4_linear: bias", bias, n)
     _same_device("mx4_linear", xt, w.data, bias)
-    lead = x.shape[:-1]
+    lead = xt.shape[:-1]
     rows = xt.numel() // xt.shape[-1]
     if not mx and rows > _MX4_WIDEN_ROWS:
         # many rows: the weights are read by many workgroups, so widening them once costs less than in every one of them
@@ -1146,7 +1151,7 @@ def mx4_linear_dgrad(dy: torch.Tensor, w: MxTensor) -> torch.Tensor:
     if rows == 0:
         return torch.empty((*dy.shape[:-1], k), dtype=dy.dtype, device=dy.device)
     np_ = (n + 7) // 8 * 8
-    wt = torch.empty((k, np_), dtype=torch.bfloat16, device=dy.device)
+    wt = torch.empty((k, np_), dtype=dy.dtype, device=dy.device)
     _call(dy, "ldm_mx4_dequantize_t", w.data.data_ptr(), w.scale.data_ptr(), n, k, wt.data_ptr(), np_)
     return _linear_bf16(dy.reshape(rows, n), wt, None, torch.bfloat16).view(*dy.shape[:-1], k)
 
@@ -1182,12 +1187,12 @@ def glu_backward_mx8(h8: MxTensor, dout: torch.Tensor, act: str, recompute: bool
     _gpu(dout)
     code = dt_code(dout.dtype)
     _same_dtype_dense("glu_backward_mx8", dout)
-    if h8.cols % 32 or tuple(dout.shape) != (*h8.shape[:-1], h8.cols // 2):
+    if h8.cols % 32 or dout.dim() < 1 or dout.shape[-1] != h8.cols // 2 or dout.shape[:-1] != h8.data.shape[:-1]:
         raise ValueError(f"glu_backward_mx8: dout {tuple(dout.shape)} does not match the checkpoint {tuple(h8.shape)}")
     _same_device("glu_backward_mx8", dout, h8.data)
     ff = h8.cols // 2
-    dh = torch.empty(tuple(h8.shape), dtype=dout.dtype, device=dout.device)
-    out = torch.empty(tuple(dout.shape), dtype=dout.dtype, device=dout.device) if recompute else None
+    dh = torch.empty((*dout.shape[:-1], h8.cols), dtype=dout.dtype, device=dout.device)
+    out = torch.empty(dout.shape, dtype=dout.dtype, device=dout.device) if recompute else None
     _call(dout, "ldm_glu_backward_mx8", h8.data.data_ptr(), h8.scale.data_ptr(), dout.data_ptr(), dh.data_ptr(), _ptr(out), code, h8.rows,
           ff, gelu)
     return (dh, out) if recompute else dh
@@ -1200,7 +1205,7 @@ def linear_wgrad_mx8(x8: MxTensor, dy: torch.Tensor, *, out: Optional[torch.Tens
     _gpu(dy, out)
     if dy.dtype != torch.bfloat16:
         raise TypeError(f"linear_wgrad_mx8: dy must be bfloat16 (got {dy.dtype})")
-    if dy.dim() < 1 or dy.shape[-1] < 1 or dy.shape[:-1] != x8.shape[:-1] or not dy.is_contiguous():
+    if dy.dim() < 1 or dy.shape[-1] < 1 or dy.shape[:-1] != x8.data.shape[:-1] or not dy.is_contiguous():
         raise ValueError(f"linear_wgrad_mx8: dy must be a contiguous {(*x8.shape[:-1], 'n')} tensor, got {tuple(dy.shape)}")
     _same_device("linear_wgrad_mx8", dy, x8.data, out)
     n, k, rows = dy.shape[-1], x8.cols, x8.rows
