@@ -5,7 +5,7 @@
 // Both operands mx4: v_mfma_scale_f32_32x32x64_f8f6f4.  A lane's operand is 32 consecutive k of one row -- one block, 16 bytes as stored --
 // and its scale byte; products and sums are float32 inside the instruction, so nothing is rounded before the output.  The weights
 // are the instruction's first operand: a lane then holds four consecutive n of one m.
-//   mx4_gemm_kernel   large outputs.  8192^3: 325-345 us, 3.2-3.4 PFLOP/s (a loop of this instruction alone on random operands, without
+//   mx4_gemm_kernel   large outputs.  8192^3: 310-340 us, 3.2-3.5 PFLOP/s (a loop of this instruction alone on random operands, without
 //                     any loads: 6.4); 32768 x 2560, k = 320: 52 us, 168 MB of output at 3.2 TB/s.
 //   mx_gemm_kernel    small and medium outputs, and plain bf16 operands (the product behind the widening of the weights): 8192 x 640, k =
 //                     5120 in bf16: 66 us, 810 TFLOP/s; 154 x 768, k = 1312: 6.9 us.
@@ -151,12 +151,12 @@ __device__ __forceinline__ void store_tiles(const Mx4Params& p, const f32x16_t (
 // Scales: one 32-bit word a row and step.  From four steps on, 16 bytes (four steps) a row at a time in one DMA instruction, the last
 // ones ending with the row (a fetch never passes its row); with fewer steps word by word, once.
 template <int BM, int BN, int WM, int WN, int S, typename OUT>
-__global__ void __launch_bounds__(64 * WM * WN)
+__global__ void __launch_bounds__(64 * WM * WN, 2)
 mx4_gemm_kernel(const Mx4Params p) {
   constexpr int NT = 64 * WM * WN, ROWS = BM + BN;
   constexpr int IT = ROWS * 4 / NT;                        // tile DMA instructions of a wave a step
-  constexpr int SIT = ROWS / NT;                           // scale DMA instructions of a wave (16 bytes a row)
-  static_assert(BM * 4 % NT == 0 && BN * 4 % NT == 0 && ROWS % NT == 0 && BM % 64 == 0, "tile / threads mismatch");
+  constexpr int SIT = (ROWS + NT - 1) / NT;                // scale DMA instructions of a wave (16 bytes a row)
+  static_assert(BM * 4 % NT == 0 && BN * 4 % NT == 0 && BM % 64 == 0 && BN % 64 == 0, "tile / threads mismatch");
   constexpr int STAGE = ROWS * 64;
   constexpr int SCALES = ROWS * 16;              // one group of four steps
   constexpr int WTM = BM / WM, WTN = BN / WN, MI = WTM / 32, NI = WTN / 32;
@@ -208,6 +208,7 @@ mx4_gemm_kernel(const Mx4Params p) {
 #pragma unroll
         for (int it = 0; it < SIT; ++it) {
           const int r0 = it * NT + wave * 64, row = r0 + lane;
+          if (r0 >= ROWS) continue;
           if (r0 < BM) mx_dma4(xsbase, xsbytes, dst + (j * ROWS + r0) * 4, (unsigned)row * p.sstride, j * 4);
           else mx_dma4(wsbase, wsbytes, dst + (j * ROWS + r0) * 4, (unsigned)(row - BM) * p.sstride, j * 4);
         }
@@ -216,6 +217,7 @@ mx4_gemm_kernel(const Mx4Params p) {
 #pragma unroll
       for (int it = 0; it < SIT; ++it) {
         const int r0 = it * NT + wave * 64, row = r0 + lane;
+        if (r0 >= ROWS) continue;
         if (r0 < BM) mx_dma16(xsbase, xsbytes, dst + r0 * 16, (unsigned)row * p.sstride, first);
         else mx_dma16(wsbase, wsbytes, dst + r0 * 16, (unsigned)(row - BM) * p.sstride, first);
       }
@@ -863,6 +865,9 @@ static int mx4_linear_out(Mx4Params& p, bool mx, hipStream_t st) {
   const float a = tile_rounds(p, 64, 64) * 0.55f, b = tile_rounds(p, 128, 128), c = tile_rounds(p, 256, 256) * 2.3f;
   if (a <= b && a <= c) return launch_mx_gemm<64, 64, 1, 1, 4, 2, true, OUT>(p, st);
   if (b <= c) return launch_mx_gemm<128, 128, 2, 2, 1, 3, true, OUT>(p, st);
+  // Short sums: two workgroups a CU, one's output and first loads behind the other's products (8192 x 5120, k = 640: 34.3 us against 37.2,
+  // 2048 x 10240, k = 1280: 31.0 / 32.9); long ones: the larger tile's fewer operand reads (k = 4096: 52.3 / 49.8, 8192: 353 / 310).
+  if (p.k < 2048) return launch_mx4_gemm<256, 128, 2, 2, 2, OUT>(p, st);
   return launch_mx4_gemm<256, 256, 2, 4, 4, OUT>(p, st);
 }
 

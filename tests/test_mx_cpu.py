@@ -115,9 +115,15 @@ def test_product_few_rows_wide_and_unaligned():
 @pytest.mark.parametrize("dma", ["lazy", "eager"])
 @pytest.mark.parametrize("rows,n,k", [(66, 200, 2100), (130, 70, 777), (1100, 1300, 300), (1030, 1410, 1100), (2050, 4104, 200)])
 def test_product_both_4bit_tiles(rows, n, k, dma):
-    """Outputs of every tile's choice -- 64 x 64 with its columns split, 128 x 128, 256 x 256 -- with more steps than LDS has slots."""
+    """Outputs of every tile's choice -- 64 x 64 with its columns split, 128 x 128, 256 x 128 -- with more steps than LDS has slots."""
     with Guarded() as g, emulated(dma, guard=True) as ops:
         mx.check_linear(ops, rows, n, k, 21, "mx4", bf if n % 4 else torch.float32, True, g.like)
+
+
+def test_product_both_4bit_largest_tile():
+    """256 x 256: many outputs and long sums."""
+    with Guarded() as g, emulated("lazy", guard=True) as ops:
+        mx.check_linear(ops, 2050, 4104, 2050, 21, "mx4", bf, True, g.like)
 
 
 @pytest.mark.parametrize("dma", ["lazy", "eager"])

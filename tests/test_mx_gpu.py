@@ -83,9 +83,9 @@ def test_product_many_bf16_rows(rows, n, k):
     mx.check_linear(ops, rows, n, k, 15, "bf16", bf, True, dev)
 
 
-@pytest.mark.parametrize("rows,n,k", [(66, 200, 2100), (130, 70, 7777), (1100, 1300, 300), (1030, 1410, 4100), (2050, 4104, 2000)])
+@pytest.mark.parametrize("rows,n,k", [(66, 200, 2100), (130, 70, 7777), (1100, 1300, 300), (1030, 1410, 4100), (2050, 4104, 2000), (2050, 4104, 2050), (4100, 4000, 3000)])
 def test_product_both_4bit_tiles(rows, n, k):
-    """Outputs of every tile's choice -- 64 x 64 with its columns split, 128 x 128, 256 x 256 -- with more steps than LDS has slots."""
+    """Outputs of every tile's choice -- 64 x 64 with its columns split, 128 x 128, 256 x 128, 256 x 256 -- with more steps than LDS has slots."""
     mx.check_linear(ops, rows, n, k, 21, "mx4", bf if n % 4 else torch.float32, True, dev)
 
 
