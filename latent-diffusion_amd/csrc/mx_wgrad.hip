@@ -13,9 +13,9 @@
 // rows are split over workgroups where there are few tiles; the partial tiles are added by a second kernel in a fixed order (no
 // atomics).
 //
-// 32768 rows, 2560 x 320 (54 GFLOP, 180 MB): 70 us + 12 us for the 16 partial tiles, 650 TFLOP/s; a large bf16 matrix product reaches
-// 1170.  What is left between: LDS (the transposed reads of a step take 0.8 of its matrix time, dY's arrival and the widened
-// image 0.4 more), and 52 MB of partial tiles written and read.
+// 32768 rows, 2560 x 320 (54 GFLOP, 180 MB): 68 us + 9 us for the 16 partial tiles, 700 TFLOP/s; a large bf16 matrix product reaches
+// 1220.  Parts left out one at a time: the partial tiles' stores 10 us, dY's loads 13, the widening 2 (6 without dY's loads), the
+// fragments' reads 4; the products alone take 26.
 #include "common.h"
 
 #include <type_traits>
