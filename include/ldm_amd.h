@@ -460,6 +460,16 @@ int ldm_pad_columns_bf16(const void* x, void* out, long long rows, int cols, int
  * 2^21: the product behind ldm_mx_dequantize / ldm_mx4_dequantize_t, for many rows.  bias, out, sums as above. */
 int ldm_linear_bf16(const void* x, const void* w, const float* bias, void* out, int out_dtype, long long rows, int n, int k, void* stream);
 
+/* Many rows of bfloat16 on LDM_MX4 weights (n, k): the weights are widened once into the workspace, then ldm_linear_bf16.
+ *   wide:  out (rows, n) = x W^T + bias, x (rows, k); inner = k (at most 2^21), outer = n
+ *   dgrad: dx (rows, k) bfloat16 = dY W, dY (rows, n); inner = n (at most 2^21), outer = k
+ * x / dY: contiguous bfloat16 at any alignment.  Workspace (16-byte aligned): 2 * inner8 * (outer + rows) bytes with inner8 = inner rounded up
+ * to a multiple of 8; without `rows` where inner is one and x / dY is 16-byte aligned. */
+int ldm_mx4_linear_wide(const void* x, const void* w, const void* w_scale, const float* bias, void* out, int out_dtype, long long rows,
+                        int n, int k, void* workspace, long long workspace_bytes, void* stream);
+int ldm_mx4_linear_dgrad(const void* dy, const void* w, const void* w_scale, void* dx, long long rows, int n, int k, void* workspace,
+                         long long workspace_bytes, void* stream);
+
 /* dw (n, k) float32 (+)= dY^T X: weight gradient of a linear layer whose input was kept in LDM_MX8.  dy (rows, n) bfloat16, contiguous,
  * 16-byte aligned, n a multiple of 8; x8 / x8_scale (rows, k).  Sums are float32 in a fixed order (no atomics).  `workspace` of
  * ldm_linear_wgrad_mx8_workspace_bytes (may be 0: NULL is fine then), 16-byte aligned. */

@@ -935,3 +935,50 @@ extern "C" int ldm_linear_bf16(const void* x, const void* w, const float* bias, 
   LDM_HIP_CHECK_LAUNCH("ldm_linear_bf16");
   return LDM_OK;
 }
+
+// *x: rows that the product can fetch, in the front of the workspace if they have to be laid out for it; *wide: the place of the widened weights
+// behind them.  Everything that the steps after this one could refuse has been looked at: a refused call launches nothing.
+static int mx_rows_for_product(const char* what, const void** x, const void* w, const void* w_scale, const void* bias, const void* out, int out_dtype,
+                               long long rows, int cols, int ld, long long outer, void* workspace, long long workspace_bytes, void** wide, void* stream) {
+  LDM_REQUIRE(dtype_ok(out_dtype), "%s: bad dtype %d", what, out_dtype);
+  LDM_REQUIRE(*x && w && w_scale && out && (reinterpret_cast<uintptr_t>(*x) & 1) == 0 && aligned16(w) &&
+                  (reinterpret_cast<uintptr_t>(w_scale) & 3) == 0 && (reinterpret_cast<uintptr_t>(bias) & 3) == 0 &&
+                  reinterpret_cast<uintptr_t>(out) % dtype_size(out_dtype) == 0,
+              "%s: null or unaligned pointer", what);
+  LDM_REQUIRE(rows < (1LL << 40) && outer <= (1 << 30) && ((rows + 63) / 64) * ((outer + 63) / 64) < (1LL << 31), "%s: %lld x %lld outputs are too many",
+              what, rows, outer);
+  const bool pad = ld != cols || !aligned16(*x);
+  const long long need = (outer + (pad ? rows : 0)) * ld * 2;
+  LDM_REQUIRE(workspace != nullptr && aligned16(workspace) && workspace_bytes >= need, "%s: workspace of %lld bytes needed (got %lld)", what, need,
+              workspace_bytes);
+  *wide = workspace;
+  if (!pad) return LDM_OK;
+  const int rc = ldm_pad_columns_bf16(*x, workspace, rows, cols, ld, stream);
+  *x = workspace;
+  *wide = static_cast<bf16_t*>(workspace) + rows * ld;
+  return rc;
+}
+
+extern "C" int ldm_mx4_linear_wide(const void* x, const void* w, const void* w_scale, const float* bias, void* out, int out_dtype, long long rows, int n,
+                                   int k, void* workspace, long long workspace_bytes, void* stream) {
+  LDM_REQUIRE(rows >= 0 && n >= 1 && k >= 1 && k <= (1 << 21), "ldm_mx4_linear_wide: bad sizes (rows=%lld n=%d k=%d)", rows, n, k);
+  if (rows == 0) return LDM_OK;
+  const int kp = (k + 7) & ~7;
+  void* wide = nullptr;
+  if (int rc = mx_rows_for_product("ldm_mx4_linear_wide", &x, w, w_scale, bias, out, out_dtype, rows, k, kp, n, workspace, workspace_bytes, &wide, stream))
+    return rc;
+  if (int rc = ldm_mx_dequantize(w, w_scale, LDM_MX4, n, kp, wide, LDM_BF16, kp, stream)) return rc;
+  return ldm_linear_bf16(x, wide, bias, out, out_dtype, rows, n, kp, stream);
+}
+
+extern "C" int ldm_mx4_linear_dgrad(const void* dy, const void* w, const void* w_scale, void* dx, long long rows, int n, int k, void* workspace,
+                                    long long workspace_bytes, void* stream) {
+  LDM_REQUIRE(rows >= 0 && n >= 1 && n <= (1 << 21) && k >= 1, "ldm_mx4_linear_dgrad: bad sizes (rows=%lld n=%d k=%d)", rows, n, k);
+  if (rows == 0) return LDM_OK;
+  const int np = (n + 7) & ~7;
+  void* wide = nullptr;
+  if (int rc = mx_rows_for_product("ldm_mx4_linear_dgrad", &dy, w, w_scale, nullptr, dx, LDM_BF16, rows, n, np, k, workspace, workspace_bytes, &wide, stream))
+    return rc;
+  if (int rc = ldm_mx4_dequantize_t(w, w_scale, n, k, wide, np, stream)) return rc;
+  return ldm_linear_bf16(dy, wide, nullptr, dx, LDM_BF16, rows, k, np, stream);
+}

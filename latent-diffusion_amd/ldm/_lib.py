@@ -130,6 +130,9 @@ _SIGNATURES = {
     "ldm_mx4_linear": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, C.c_longlong, c_int, c_int, c_void_p],
     "ldm_pad_columns_bf16": [c_void_p, c_void_p, C.c_longlong, c_int, c_int, c_void_p],
     "ldm_linear_bf16": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, C.c_longlong, c_int, c_int, c_void_p],
+    "ldm_mx4_linear_wide": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, C.c_longlong, c_int, c_int, c_void_p, C.c_longlong,
+                            c_void_p],
+    "ldm_mx4_linear_dgrad": [c_void_p, c_void_p, c_void_p, c_void_p, C.c_longlong, c_int, c_int, c_void_p, C.c_longlong, c_void_p],
     "ldm_linear_wgrad_mx8": [c_void_p, c_void_p, c_void_p, c_void_p, C.c_longlong, c_int, c_int, c_int, c_void_p, C.c_longlong,
                              c_void_p],
 }

@@ -1083,13 +1083,12 @@ def _pad_cols(t: torch.Tensor, cols: int) -> torch.Tensor:
     return out
 
 
-def _linear_bf16(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], out_dtype: torch.dtype) -> torch.Tensor:
-    """x (rows, k) W^T + bias for widened weights w (n, k rounded up to 8)."""
-    rows, (n, kp) = x.shape[0], w.shape
-    x = _pad_cols(x, kp)
-    out = torch.empty((rows, n), dtype=out_dtype, device=x.device)
-    _call(x, "ldm_linear_bf16", x.data_ptr(), w.data_ptr(), _ptr(bias), out.data_ptr(), dt_code(out_dtype), rows, n, kp)
-    return out
+def _widening_workspace(x: torch.Tensor, rows: int, inner: int, outer: int):
+    """(workspace, bytes) of ldm_mx4_linear_wide / ldm_mx4_linear_dgrad: the widened weights, and x's rows where they cannot be fetched 16
+    bytes at a time."""
+    inner8 = (inner + 7) // 8 * 8
+    size = inner8 * (outer + (rows if inner8 != inner or x.data_ptr() % 16 else 0))
+    return torch.empty(size, dtype=torch.bfloat16, device=x.device), 2 * size
 
 
 def mx4_linear(x, w: MxTensor, bias: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
@@ -1123,10 +1122,11 @@ def mx4_linear(x, w: MxTensor, bias: Optional[torch.Tensor] = None, out_dtype: O
     rows = xt.numel() // xt.shape[-1]
     if not mx and rows > _MX4_WIDEN_ROWS:
         # many rows: the weights are read by many workgroups, so widening them once costs less than in every one of them
-        kp = (k + 7) // 8 * 8
-        wide = torch.empty((n, kp), dtype=torch.bfloat16, device=x.device)
-        _call(x, "ldm_mx_dequantize", w.data.data_ptr(), w.scale.data_ptr(), _lib.MX4, n, kp, wide.data_ptr(), BF16, kp)
-        return _linear_bf16(x.reshape(rows, k), wide, bias, odt).view(*lead, n)
+        out = torch.empty((*lead, n), dtype=odt, device=x.device)
+        ws, need = _widening_workspace(x, rows, k, n)
+        _call(x, "ldm_mx4_linear_wide", x.data_ptr(), w.data.data_ptr(), w.scale.data_ptr(), _ptr(bias), out.data_ptr(), code, rows, n, k,
+              ws.data_ptr(), need)
+        return out
     out = torch.empty((*lead, n), dtype=odt, device=xt.device)
     if rows:
         _call(xt, "ldm_mx4_linear", xt.data_ptr(), x.scale.data_ptr() if mx else 0, w.data.data_ptr(), w.scale.data_ptr(), _ptr(bias),
@@ -1141,19 +1141,18 @@ def mx4_linear_dgrad(dy: torch.Tensor, w: MxTensor) -> torch.Tensor:
     if w.data.dim() != 2:
         raise ValueError(f"mx4_linear_dgrad: w must be (n, k), got {tuple(w.shape)}")
     _gpu(dy)
-    n, k = w.shape
+    n, k = w.data.shape[0], w.cols
     if dy.dtype != torch.bfloat16:
         raise TypeError(f"mx4_linear_dgrad: dy must be bfloat16 (got {dy.dtype})")
     if dy.dim() < 1 or dy.shape[-1] != n or not dy.is_contiguous():
         raise ValueError(f"mx4_linear_dgrad: dy must be a contiguous (..., {n}) tensor, got {tuple(dy.shape)}")
     _same_device("mx4_linear_dgrad", dy, w.data)
     rows = dy.numel() // n
-    if rows == 0:
-        return torch.empty((*dy.shape[:-1], k), dtype=dy.dtype, device=dy.device)
-    np_ = (n + 7) // 8 * 8
-    wt = torch.empty((k, np_), dtype=dy.dtype, device=dy.device)
-    _call(dy, "ldm_mx4_dequantize_t", w.data.data_ptr(), w.scale.data_ptr(), n, k, wt.data_ptr(), np_)
-    return _linear_bf16(dy.reshape(rows, n), wt, None, torch.bfloat16).view(*dy.shape[:-1], k)
+    out = torch.empty((*dy.shape[:-1], k), dtype=dy.dtype, device=dy.device)
+    if rows:
+        ws, need = _widening_workspace(dy, rows, n, k)
+        _call(dy, "ldm_mx4_linear_dgrad", dy.data_ptr(), w.data.data_ptr(), w.scale.data_ptr(), out.data_ptr(), rows, n, k, ws.data_ptr(), need)
+    return out
 
 
 def _glu_kind(what: str, act: str) -> int:

@@ -326,6 +326,21 @@ def test_c_entries_refuse_without_a_launch():
     assert bad(lib.ldm_linear_bf16(p, p, 0, p, 5, 1, 1, 8, 0))
     assert bad(lib.ldm_linear_bf16(p, p, 0, p, 1, 1 << 39, 1 << 30, 8, 0))
     assert lib.ldm_linear_bf16(0, 0, 0, 0, 1, 0, 1, 8, 0) == 0
+    assert bad(lib.ldm_mx4_linear_wide(p, p, p, 0, p, 1, 1, 8, 8, p, 127, 0))                 # 2 * 8 * 8 bytes of workspace
+    assert bad(lib.ldm_mx4_linear_wide(p, p, p, 0, p, 1, 1, 8, 8, 0, 128, 0))
+    assert bad(lib.ldm_mx4_linear_wide(p, p, p, 0, p, 1, 1, 8, 7, p, 128, 0))                 # and 2 * 8 for the row laid out anew
+    assert bad(lib.ldm_mx4_linear_wide(p, 0, p, 0, p, 1, 1, 8, 7, p, 4096, 0))                # nothing launched for the rows either
+    assert bad(lib.ldm_mx4_linear_wide(p, p, p, 0, p + 1, 1, 1, 8, 7, p, 4096, 0))
+    assert bad(lib.ldm_mx4_linear_wide(p, p, p, 0, p, 7, 1, 8, 7, p, 4096, 0))
+    assert bad(lib.ldm_mx4_linear_dgrad(p, p, 0, p, 1, 7, 8, p, 4096, 0))
+    assert bad(lib.ldm_mx4_linear_wide(p, p, p + 2, 0, p, 1, 1, 8, 7, p, 4096, 0))
+    assert bad(lib.ldm_mx4_linear_wide(p + 1, p, p, 0, p, 1, 1, 8, 8, p, 4096, 0))
+    assert bad(lib.ldm_mx4_linear_wide(p, p, p, 0, p, 1, 1, 8, (1 << 21) + 1, p, 4096, 0))
+    assert lib.ldm_mx4_linear_wide(0, 0, 0, 0, 0, 1, 0, 8, 8, 0, 0, 0) == 0
+    assert bad(lib.ldm_mx4_linear_dgrad(p, p, p, p, 1, 8, 8, p, 127, 0))
+    assert bad(lib.ldm_mx4_linear_dgrad(p + 2, p, p, p, 1, 8, 8, p, 128, 0))
+    assert bad(lib.ldm_mx4_linear_dgrad(p, p, p, p, 1, 0, 8, p, 4096, 0))
+    assert lib.ldm_mx4_linear_dgrad(0, 0, 0, 0, 0, 8, 8, 0, 0, 0) == 0
     assert bad(lib.ldm_pad_columns_bf16(p, p, 1, 8, 12, 0))
     assert bad(lib.ldm_pad_columns_bf16(p, p, 1, 9, 8, 0))
     assert bad(lib.ldm_pad_columns_bf16(p + 1, p, 1, 7, 8, 0))
