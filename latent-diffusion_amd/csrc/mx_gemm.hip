@@ -859,7 +859,9 @@ static float tile_rounds(const Mx4Params& p, int bm, int bn) {
 template <typename OUT>
 static int mx4_linear_out(Mx4Params& p, bool mx, hipStream_t st) {
   if (!mx) return p.k % 8 == 0 && aligned16(p.x) ? rows_by_size<false, true, OUT>(p, st) : rows_by_size<false, false, OUT>(p, st);
-  if (p.rows <= 64) return rows_by_size<true, true, OUT>(p, st);
+  // few rows, or few enough outputs that each CU has at most one workgroup of the few-row kernel: 128 x 1280 (k = 1280) 3.5 us against 5.9 in
+  // tiles; with more, its re-reading of the operands loses: 128 x 10240 (k = 1280) 10.4 / 8.7
+  if (p.rows <= 64 || ((p.rows + 63) / 64) * ((p.n + 15) / 16) <= 256) return rows_by_size<true, true, OUT>(p, st);
   // rounds of one workgroup a CU x the time of 256 columns of the tile (us: 64 x 64 with its columns split 0.55, 128 x 128 1, 256 x 256
   // 2.3).  8192^3: 715, 464 and 341 us; 2048^3: 21.5, 11.5, 12.3; 154 x 2560 (k = 2560): 7.3, 10.4, 12.0
   const float a = tile_rounds(p, 64, 64) * 0.55f, b = tile_rounds(p, 128, 128), c = tile_rounds(p, 256, 256) * 2.3f;

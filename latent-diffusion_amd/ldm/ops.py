@@ -1071,7 +1071,11 @@ def mx_dequantize(q: MxTensor, dtype: torch.dtype) -> torch.Tensor:
     return out
 
 
-_MX4_WIDEN_ROWS = 64        # bf16 activations: up to here the weights are widened in registers, beyond once to memory
+def _mx4_widen_once(rows: int, n: int) -> bool:
+    """bf16 activations: whether the weights are widened once to memory, or in registers, by workgroups of 64 rows and 16 outputs.
+    In registers up to 256 rows (1280 on 10240 outputs: 24.9 us against 29.2; 384 rows 36.9 / 29.0), and while such workgroups are few
+    (512 rows of 1280 on 320 outputs 5.9 / 12.3, on 1280 outputs 12.8 / 14.2; 2560 on 2560 28.7 / 28.6)."""
+    return rows > 256 and ((rows + 63) // 64) * ((n + 15) // 16) > 960
 
 
 def _pad_cols(t: torch.Tensor, cols: int) -> torch.Tensor:
@@ -1120,8 +1124,7 @@ def mx4_linear(x, w: MxTensor, bias: Optional[torch.Tensor] = None, out_dtype: O
     _same_device("mx4_linear", xt, w.data, bias)
     lead = xt.shape[:-1]
     rows = xt.numel() // xt.shape[-1]
-    if not mx and rows > _MX4_WIDEN_ROWS:
-        # many rows: the weights are read by many workgroups, so widening them once costs less than in every one of them
+    if not mx and _mx4_widen_once(rows, n):
         out = torch.empty((*lead, n), dtype=odt, device=x.device)
         ws, need = _widening_workspace(x, rows, k, n)
         _call(x, "ldm_mx4_linear_wide", x.data_ptr(), w.data.data_ptr(), w.scale.data_ptr(), _ptr(bias), out.data_ptr(), code, rows, n, k,

@@ -127,7 +127,7 @@ def test_product_both_4bit_largest_tile():
 
 
 @pytest.mark.parametrize("dma", ["lazy", "eager"])
-@pytest.mark.parametrize("rows,n,k", [(66, 130, 1300), (70, 33, 8), (1030, 1000, 200), (500, 10230, 200), (1000, 10230, 200)])
+@pytest.mark.parametrize("rows,n,k", [(300, 3200, 200), (1300, 1000, 77), (300, 130, 1300), (66, 130, 1300), (70, 33, 8), (1030, 1000, 200), (500, 10230, 200), (1000, 10230, 200)])
 def test_product_bf16_tiles(rows, n, k, dma):
     """Likewise for bfloat16 activations: 64 x 64, 128 x 128, 128 x 160, 256 x 160."""
     with Guarded() as g, emulated(dma, guard=True) as ops:

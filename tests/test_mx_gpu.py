@@ -89,7 +89,7 @@ def test_product_both_4bit_tiles(rows, n, k):
     mx.check_linear(ops, rows, n, k, 21, "mx4", bf if n % 4 else torch.float32, True, dev)
 
 
-@pytest.mark.parametrize("rows,n,k", [(66, 130, 1300), (70, 33, 8), (154, 1290, 5001), (1030, 1000, 2000), (500, 10230, 1000), (1000, 10230, 1000)])
+@pytest.mark.parametrize("rows,n,k", [(300, 3200, 200), (1300, 1000, 77), (300, 130, 1300), (66, 130, 1300), (70, 33, 8), (154, 1290, 5001), (1030, 1000, 2000), (500, 10230, 1000), (1000, 10230, 1000)])
 def test_product_bf16_tiles(rows, n, k):
     """Likewise for bfloat16 activations: 64 x 64, 128 x 128, 128 x 160, 256 x 160."""
     mx.check_linear(ops, rows, n, k, 22, "bf16", bf if n % 3 else torch.float32, True, dev)
