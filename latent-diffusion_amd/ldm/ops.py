@@ -1200,6 +1200,14 @@ def glu_backward_mx8(h8: MxTensor, dout: torch.Tensor, act: str, recompute: bool
     return (dh, out) if recompute else dh
 
 
+def _wgrad_mx8(x8: MxTensor, dy: torch.Tensor, out: torch.Tensor, rows: int, n: int, k: int, accumulate: int) -> None:
+    need = _lib.load().ldm_linear_wgrad_mx8_workspace_bytes(rows, n, k)
+    # from the allocator, not kept: a graph that captured the call owns its own, and no other call or graph writes to it
+    ws = torch.empty(need, dtype=torch.uint8, device=dy.device) if need else None
+    _call(dy, "ldm_linear_wgrad_mx8", x8.data.data_ptr(), x8.scale.data_ptr(), dy.data_ptr(), out.data_ptr(), rows, n, k, accumulate, _ptr(ws),
+          need)
+
+
 def linear_wgrad_mx8(x8: MxTensor, dy: torch.Tensor, *, out: Optional[torch.Tensor] = None, accumulate: Optional[bool] = None) -> torch.Tensor:
     """Weight gradient dY^T X (n, k) float32 of a linear layer whose input was kept as an 8-bit checkpoint x8 (*lead, k); dy (*lead, n)
     bfloat16.  ``out`` / ``accumulate`` as conv_wgrad: an existing gradient to accumulate into, or a buffer to overwrite."""
@@ -1216,15 +1224,13 @@ def linear_wgrad_mx8(x8: MxTensor, dy: torch.Tensor, *, out: Optional[torch.Tens
     accumulate = out is not None and (accumulate is None or bool(accumulate))
     npad = (n + 7) // 8 * 8
     if rows and (npad != n or dy.data_ptr() % 16):      # the kernel fetches dy in 16-byte pieces: other rows go through a padded copy
-        full = linear_wgrad_mx8(x8, _pad_cols(dy.reshape(rows, n), npad).view(*dy.shape[:-1], npad))[:n]
+        full = torch.empty((npad, k), dtype=torch.float32, device=dy.device)
+        _wgrad_mx8(x8, _pad_cols(dy.view(rows, n), npad), full, rows, npad, k, 0)
+        full = full[:n]
         return full if out is None else out.add_(full) if accumulate else out.copy_(full)
     if out is None:
         out = torch.empty((n, k), dtype=torch.float32, device=dy.device)
     if rows == 0:
         return out if accumulate else out.zero_()
-    need = _lib.load().ldm_linear_wgrad_mx8_workspace_bytes(rows, n, k)
-    # from the allocator, not kept: a graph that captured the call owns its own, and no other call or graph writes to it
-    ws = torch.empty(need, dtype=torch.uint8, device=dy.device) if need else None
-    _call(dy, "ldm_linear_wgrad_mx8", x8.data.data_ptr(), x8.scale.data_ptr(), dy.data_ptr(), out.data_ptr(), rows, n, k,
-          1 if accumulate else 0, _ptr(ws), need)
+    _wgrad_mx8(x8, dy, out, rows, n, k, 1 if accumulate else 0)
     return out
