@@ -423,7 +423,8 @@ int ldm_image_to_uint8(const void* x, int dtype, unsigned char* out, long long n
  *            half: 16 bytes a block.
  *   LDM_MX8  e = max(floor(log2 a), -127); elements q / 64, q = -127 .. 127: 64 x / 2^e to nearest even, at most 127.  32 bytes a block.
  * A block that holds an infinity or a NaN gets the byte 255 and stands for NaN in all its 32 columns.  data: rows without gaps
- * (16-byte aligned); scale: rows of 4 * ceil(blocks / 4) bytes, the padding bytes zero (4-byte aligned). */
+ * (16-byte aligned); scale: rows of 4 * ceil(blocks / 4) bytes, the padding bytes zero (4-byte aligned).  No reader counts on the zeros: elements
+ * behind the last column and scale bytes behind the last block do not enter any result. */
 int ldm_mx_quantize(const void* x, int dtype, long long rows, int cols, long long ld, int fmt, void* data, void* scale, void* stream);
 
 /* The values that `data` / `scale` stand for -> out (rows, cols), rows `ld` elements apart; exact in float32 and (LDM_MX4, LDM_MX8: at

@@ -63,9 +63,44 @@ template <int OFF>
 __device__ __forceinline__ void lds_read4(int& v, unsigned addr) {
   asm volatile("ds_read_b32 %0, %1 offset:%2" : "=v"(v) : "v"(addr), "n"(OFF) : "memory");
 }
+template <int OFF>
+__device__ __forceinline__ void lds_write16(unsigned addr, i32x4_t v) {
+  asm volatile("ds_write_b128 %0, %1 offset:%2" ::"v"(addr), "v"(v), "n"(OFF) : "memory");
+}
 // no use of v moves above the wait in front of this
 __device__ __forceinline__ void stay_below(i32x4_t& v) { asm volatile("" : "+v"(v)); }
 __device__ __forceinline__ void stay_below(int& v) { asm volatile("" : "+v"(v)); }
+
+// A row's last block may be cut short, and so may its last word of scales.  What is stored behind them counts for nothing: the scale bytes
+// behind the last block are left out where a lane's byte is taken from the word, and x's elements behind the last column -- that is
+// enough, a product needs both of its factors -- are cleared in LDS once they have landed, behind branches that rows of whole blocks
+// never take (in registers, in every step or behind branches, it cost 2-9 % of all products).
+__device__ __forceinline__ unsigned scale_bytes(int blocks) { return blocks & 3 ? (1u << 8 * (blocks & 3)) - 1 : ~0u; }   // of the last word
+// selector of byte `block` of a scale word whose last block is `last` (12: zero, as is the byte behind the last block)
+__device__ __forceinline__ unsigned scale_pick(int block, int last) { return block <= last ? (unsigned)block : 12u; }
+__device__ __forceinline__ int scale_take(int word, unsigned pick) { return (int)__builtin_amdgcn_perm(0u, (unsigned)word, pick); }
+__device__ __forceinline__ int last_columns(const Mx4Params& p) { return p.k - (p.blocks - 1) * 32; }                    // of the last block
+// x's elements, in LDS: row r's last block lies at image + r PITCH + 16 (chunk ^ swizzle(r)); THREADS share the rows, those left over take the
+// last one again (which changes nothing), and the caller lets them meet afterwards
+template <int ROWS, int PITCH, int THREADS, typename SWZ>
+__device__ __forceinline__ void clear_behind(unsigned image, int chunk, int live, int thread, SWZ swizzle) {
+#pragma unroll
+  for (int r0 = 0; r0 < ROWS; r0 += THREADS) {
+    const int r = min(r0 + thread, ROWS - 1);
+    const unsigned at = image + r * PITCH + ((chunk ^ swizzle(r)) << 4);
+    i32x4_t v;
+    lds_read16<0>(v, at);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    stay_below(v);
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {                          // columns 8 d .. + 7
+      const int c = live - 8 * d;
+      v[d] &= c >= 8 ? -1 : c <= 0 ? 0 : (1 << 4 * c) - 1;
+    }
+    lds_write16<0>(at, v);
+  }
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+}
 
 template <bool MX, int H>
 __device__ __forceinline__ void mx_mfma(f32x16_t& c, i32x4_t a, i32x4_t b, int sa, int sb) {
@@ -274,7 +309,7 @@ mx4_gemm_kernel(const Mx4Params p) {
 #pragma unroll
     for (int j = 0; j < NI; ++j) lds_read4<0>(nsw[j], wsaddr + o + j * step);
   };
-  auto landed = [&]<int H>(std::integral_constant<int, H>) {
+  auto landed = [&]<int H>(std::integral_constant<int, H>, unsigned pick) {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
     for (int i = 0; i < MI; ++i) asm volatile("" : "+v"(xf[H][i]));   // no use moves above the wait
@@ -282,9 +317,9 @@ mx4_gemm_kernel(const Mx4Params p) {
     for (int j = 0; j < NI; ++j) asm volatile("" : "+v"(wf[H][j]));
     if constexpr (H == 0) {
 #pragma unroll
-      for (int i = 0; i < MI; ++i) { asm volatile("" : "+v"(nsx[i])); sx[i] = (int)((unsigned)nsx[i] >> (8 * fh)); }
+      for (int i = 0; i < MI; ++i) { asm volatile("" : "+v"(nsx[i])); sx[i] = scale_take(nsx[i], pick); }
 #pragma unroll
-      for (int j = 0; j < NI; ++j) { asm volatile("" : "+v"(nsw[j])); sw[j] = (int)((unsigned)nsw[j] >> (8 * fh)); }
+      for (int j = 0; j < NI; ++j) { asm volatile("" : "+v"(nsw[j])); sw[j] = scale_take(nsw[j], pick); }
     }
   };
   // half H of this step on the matrix cores; behind each of the first instructions a read of the other half (of `slot`)
@@ -301,6 +336,16 @@ mx4_gemm_kernel(const Mx4Params p) {
   // until this wave's DMA of the next step has landed; that of the S - 2 steps behind it may be in flight (a fetch of scales among them
   // only makes the wait stricter)
   auto dma_landed = [&] { asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 2) * IT) : "memory"); };
+  // bytes 0 and 2: this lane's scales of a step's two halves
+  const unsigned whole = scale_pick(fh, 3) | scale_pick(fh + 2, 3) << 16;
+  const unsigned ends = scale_pick(fh, (p.blocks - 1) & 3) | scale_pick(fh + 2, (p.blocks - 1) & 3) << 16;
+  auto scales_of = [&](int kt) { return kt == nk - 1 ? ends : whole; };
+  const int cut_step = (p.k & 31) ? nk - 1 : -1;
+  auto cut = [&] {                                         // the last step has landed
+    clear_behind<BM, 64, NT>(lds + (unsigned)((nk - 1) % S) * STAGE, (p.blocks - 1) & 3, last_columns(p), tid, [](int r) { return (r >> 1) & 3; });
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
   constexpr std::integral_constant<int, 0> H0{};
   constexpr std::integral_constant<int, 1> H1{};
 
@@ -309,23 +354,25 @@ mx4_gemm_kernel(const Mx4Params p) {
   dma_landed();
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
+  if (__builtin_expect(cut_step == 0, 0)) cut();
   stage(S - 1);
   read_scales(0);
   [&]<int... Q>(std::integer_sequence<int, Q...>) {
     (read(H0, std::integral_constant<int, Q>{}, 0u), ...);
   }(std::make_integer_sequence<int, READS>{});
-  landed(H0);
+  landed(H0, scales_of(0));
   for (int kt = 0; kt < nk; ++kt) {
     multiply(H0, (unsigned)(kt % S) * STAGE);
-    landed(H1);
+    landed(H1, 0u);
     const int next = min(kt + 1, nk - 1);                  // behind the last step itself once more, unused
     dma_landed();
     __builtin_amdgcn_s_barrier();                          // every wave has read slot kt, and its part of the next step is there
     asm volatile("" ::: "memory");
+    if (__builtin_expect(kt + 1 == cut_step, 0)) cut();
     stage(kt + S);
     read_scales(next);
     multiply(H1, (unsigned)(next % S) * STAGE);
-    landed(H0);
+    landed(H0, scales_of(next));
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();                                         // the slots become the epilogue's
@@ -485,7 +532,8 @@ mx_gemm_kernel(const Mx4Params p) {
     if constexpr (MX) {
 #pragma unroll
       for (int o = 0; o < 2; ++o) {
-        const unsigned there = (s0 + kt) * 2 + o < nwords ? ~0u : 0u;
+        const int word = (s0 + kt) * 2 + o;
+        const unsigned there = word < nwords - 1 ? ~0u : word == nwords - 1 ? scale_bytes(p.blocks) : 0u;
 #pragma unroll
         for (int i = 0; i < MI; ++i) { stay_below(rx[o][i]); sx[o][i] = (int)(((unsigned)rx[o][i] & there) >> (8 * fh)); }
 #pragma unroll
@@ -499,9 +547,20 @@ mx_gemm_kernel(const Mx4Params p) {
     else LDM_LOCKSTEP();
     asm volatile("" ::: "memory");
   };
+  const int cut_step = MX && (p.k & 31) ? p.nk - 1 - s0 : -1;
+  auto cut = [&](int kt) {                                 // step kt has landed
+    if constexpr (MX) {
+      if (__builtin_expect(kt != cut_step, 1)) return;
+      clear_behind<BM, 128, NT>(lds + (unsigned)(kt % S) * STAGE, (p.blocks - 1) & 7, last_columns(p), gt, [](int r) { return r & 7; });
+      if constexpr (KW == 1) __builtin_amdgcn_s_barrier();
+      else LDM_LOCKSTEP();
+      asm volatile("" ::: "memory");
+    }
+  };
   // step kt from register set SET; the next one's reads, and the DMA into the slot that is free now, between the matrix instructions
   auto step = [&]<int SET>(std::integral_constant<int, SET>, int kt) {
     next_here();
+    cut(kt + 1);
     stage_begin(kt + S);
     read_scales(kt + 1);
     const unsigned slot = (unsigned)((kt + 1) % S) * STAGE;
@@ -524,6 +583,7 @@ mx_gemm_kernel(const Mx4Params p) {
 #pragma unroll
   for (int t = 0; t < S - 1; ++t) stage(t);
   next_here();
+  cut(0);
   stage(S - 1);
   read_scales(0);
   [&]<int... Q>(std::integer_sequence<int, Q...>) {
@@ -679,6 +739,8 @@ mx4_rows_kernel(const Mx4Params p) {
   for (int s = 0; s < 4; ++s) xaddr[s] = lds + NF * 1024 + fr * 256 + (((4 * fq + s) ^ fr) << 4);
   const int sstep = word_scales ? 4 : 16;
   const unsigned saddr = lds + S * SLOT + fr * sstep;
+  const int cut_step = (p.k & 31) ? nk - 1 : -1;           // MX: a last block that is not whole
+  const unsigned whole = scale_pick(fq, 3) | 0x0c0c0c00u, ends = scale_pick(fq, (p.blocks - 1) & 3) | 0x0c0c0c00u;   // byte 0: this lane's scale
 
 #pragma unroll
   for (int s = 0; s < S - 1; ++s)
@@ -690,6 +752,12 @@ mx4_rows_kernel(const Mx4Params p) {
     const unsigned slot = (unsigned)((kt - s0) % S) * SLOT;
     const int g = (kt - s0) >> 2, word = word_scales ? 0 : kt - min(s0 + 4 * g, nk - 4);
     const unsigned sa = saddr + (g & 1) * SCALES + word * 4;
+    if constexpr (MX) {
+      if (__builtin_expect(kt == cut_step, 0)) {
+        clear_behind<16 * MT, 64, 64>(lds + slot + NF * 1024, (p.blocks - 1) & 3, last_columns(p), lane, [](int r) { return (r >> 1) & 3; });
+        LDM_LOCKSTEP();
+      }
+    }
     i32x4_t wv[NF], xv[MT][MX ? 1 : 4];
     int wc[NF], xc[MT];
 #pragma unroll
@@ -723,15 +791,16 @@ mx4_rows_kernel(const Mx4Params p) {
 #pragma unroll
       for (int s = 0; s < (MX ? 1 : 4); ++s) asm volatile("" : "+v"(xv[j][s]));
     }
+    const unsigned pick = kt == nk - 1 ? ends : whole;
 #pragma unroll
     for (int i = 0; i < NF; ++i) {
-      const unsigned code = ((unsigned)wc[i] >> (8 * fq)) & 255u;
+      const unsigned code = (unsigned)scale_take(wc[i], pick);
       if constexpr (MX) {
         const i32x8_t a{wv[i][0], wv[i][1], wv[i][2], wv[i][3], 0, 0, 0, 0};
 #pragma unroll
         for (int j = 0; j < MT; ++j) {
           const i32x8_t b{xv[j][0][0], xv[j][0][1], xv[j][0][2], xv[j][0][3], 0, 0, 0, 0};
-          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc[i][j], 4, 4, 0, (int)code, 0, (int)((unsigned)xc[j] >> (8 * fq)));
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc[i][j], 4, 4, 0, (int)code, 0, scale_take(xc[j], pick));
         }
       } else {
         const float sc = __uint_as_float(code << 23);

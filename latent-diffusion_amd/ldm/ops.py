@@ -955,8 +955,9 @@ class MxTensor:
     mx4_quantize / mx8_quantize return and what the mx operators take.
 
     data   (*lead, 16 * blocks) uint8 for 4-bit elements, (*lead, 32 * blocks) int8 for 8-bit ones, blocks = ceil(cols / 32)
-    scale  (*lead, 4 * ceil(blocks / 4)) uint8: exponent + 127 a block (255: NaN), zero behind the last block
-    cols   columns of the rows that it stands for
+    scale  (*lead, 4 * ceil(blocks / 4)) uint8: exponent + 127 a block (255: NaN)
+    cols   columns of the rows that it stands for: elements behind them and scales behind the last block count for nothing (the
+           quantisers leave zeros there)
 
     Both tensors are plain storage: they may be saved, moved or concatenated along leading dimensions like any other."""
 

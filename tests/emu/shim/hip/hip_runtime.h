@@ -227,6 +227,18 @@ static inline __attribute__((always_inline)) int update_dpp(int /*old*/, int src
   return shfl_any(src, (l & ~3) | ((ctrl >> (2 * (l & 3))) & 3), 64, 0);
 }
 
+// v_perm_b32: each byte of sel picks one of the eight bytes of (s0, s1), s1's being 0 .. 3; 12: zero (the only other value used)
+static inline unsigned perm(unsigned s0, unsigned s1, unsigned sel) {
+  const uint64_t both = (uint64_t)s0 << 32 | s1;
+  unsigned out = 0;
+  for (int i = 0; i < 4; ++i) {
+    const unsigned b = sel >> (8 * i) & 255u;
+    if (b > 7 && b != 12) abort();
+    if (b < 8) out |= (unsigned)(both >> (8 * b) & 255u) << (8 * i);
+  }
+  return out;
+}
+
 // 4-bit floats (1 sign, 2 exponent, 1 mantissa bit) under a power-of-two scale: the scale operand's exponent field is taken as it
 // is (0: 2^-127, 255: NaN); rounding to nearest even, held to 6
 static inline double e8m0(float s) {
@@ -279,6 +291,7 @@ EMU_NOINLINE C mfma_scale_fp4(A a, A b, C c, int fa, int fb, int sel_a, int sa, 
 }  // namespace emu
 
 #define __builtin_amdgcn_update_dpp ::emu::update_dpp
+#define __builtin_amdgcn_perm ::emu::perm
 #define __builtin_amdgcn_cvt_scalef32_pk_fp4_f32 ::emu::cvt_pk_fp4_f32
 #define __builtin_amdgcn_cvt_scalef32_pk_f32_fp4 ::emu::cvt_pk_f32_fp4
 #define __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4 ::emu::cvt_pk_bf16_fp4
