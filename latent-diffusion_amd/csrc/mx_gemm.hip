@@ -658,7 +658,9 @@ mx4_rows_kernel(const Mx4Params p) {
   constexpr int WAVE = S * SLOT + 2 * SCALES;
   constexpr int PER = NF + (DMAX ? XI : 0);                // LDS-DMA instructions of a step
   constexpr unsigned OOB = 0x80000000u;
-  static_assert(NF * MT * 1024 <= WAVE && S <= 6 && (S - 1) * PER < 64, "LDS image");
+  static_assert(NF * MT * 1024 <= WAVE && (S - 1) * PER < 64, "LDS image");
+  // scales have room for two groups of four steps: step 4 g + 3 fetches step 4 g + 2 + S, which must not be of group g + 2
+  static_assert(S <= 5, "scale groups");
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
