@@ -449,7 +449,9 @@ int ldm_glu_backward_mx8(const void* data, const void* scale, const void* dout, 
 /* out (rows, n) = x W^T + bias (bias float32, may be NULL; out float32 or bfloat16, contiguous), W (n, k) in LDM_MX4.
  *   x_scale != NULL: x (rows, k) in LDM_MX4 as well: both operands go to the matrix cores as they are
  *   x_scale == NULL: x (rows, k) contiguous bfloat16 (any alignment); the weights are widened to bfloat16 (exact) in registers
- * Sums are float32.  Any rows >= 0, n >= 1, 1 <= k <= 2^22.  x_scale == NULL reads W once for every 64 rows: meant for few rows. */
+ * Sums are float32.  rows >= 0 (x_scale == NULL: up to 64 * 65535), 1 <= n <= 2^30, 1 <= k <= 2^22; outputs that one launch's threads, counted
+ * in 32 bits, do not reach (2^29 columns of few rows, 2^38 outputs of many) are refused.  x_scale == NULL reads W once for every 64 rows: meant
+ * for few rows. */
 int ldm_mx4_linear(const void* x, const void* x_scale, const void* w, const void* w_scale, const float* bias, void* out, int out_dtype,
                    long long rows, int n, int k, void* stream);
 
@@ -458,7 +460,7 @@ int ldm_mx4_linear(const void* x, const void* x_scale, const void* w, const void
 int ldm_pad_columns_bf16(const void* x, void* out, long long rows, int cols, int ld, void* stream);
 
 /* out (rows, n) = x W^T + bias for plain bfloat16 operands x (rows, k), w (n, k), contiguous, 16-byte aligned, k a multiple of 8 up to
- * 2^21: the product behind ldm_mx_dequantize / ldm_mx4_dequantize_t, for many rows.  bias, out, sums as above. */
+ * 2^21: the product behind ldm_mx_dequantize / ldm_mx4_dequantize_t, for many rows.  bias, out, sums, limits of n and of outputs as above. */
 int ldm_linear_bf16(const void* x, const void* w, const float* bias, void* out, int out_dtype, long long rows, int n, int k, void* stream);
 
 /* Many rows of bfloat16 on LDM_MX4 weights (n, k): the weights are widened once into the workspace, then ldm_linear_bf16.

@@ -866,6 +866,11 @@ static int mx_allow_lds(const char* what, K kern, int bytes, bool& done) {
   return LDM_OK;
 }
 
+// A launch's threads are counted in 32 bits.
+static bool mx_launchable(long long workgroups, int threads) { return workgroups * threads < (1LL << 32); }
+// The tile kernels launch no more than tiles of 128 x 128 by 256 threads would: smaller tiles are taken only where there are few.
+static bool mx_tiles_launchable(long long rows, long long n) { return mx_launchable(((rows + 127) / 128) * ((n + 127) / 128), 256); }
+
 template <int BM, int BN, int WM, int WN, int S, typename OUT>
 static int launch_mx4_gemm(Mx4Params& p, hipStream_t st) {
   p.tiles_m = (int)((p.rows + BM - 1) / BM);
@@ -896,10 +901,12 @@ static int launch_mx_gemm(Mx4Params& p, hipStream_t st) {
 template <bool MX, int MT, int NF, int NW, int S, bool DMAX, typename OUT>
 static int launch_mx4_rows(const Mx4Params& p, hipStream_t st) {
   constexpr int smem = NW * (S * (NF + (MX ? MT : 4 * MT)) * 1024 + (MX ? 4096 : 2048));
+  const dim3 grid((p.n + 16 * NF - 1) / (16 * NF), (unsigned)((p.rows + 16 * MT - 1) / (16 * MT)));
+  LDM_REQUIRE(mx_launchable((long long)grid.x * grid.y, 64 * NW), "ldm_mx4_linear: %lld x %d outputs are too many", p.rows, p.n);
   auto kern = mx4_rows_kernel<MX, MT, NF, NW, S, DMAX, OUT>;
   static bool done = false;
   if (int rc = mx_allow_lds("ldm_mx4_linear", kern, smem, done)) return rc;
-  hipLaunchKernelGGL(kern, dim3((p.n + 16 * NF - 1) / (16 * NF), (unsigned)((p.rows + 16 * MT - 1) / (16 * MT))), dim3(64 * NW), smem, st, p);
+  hipLaunchKernelGGL(kern, grid, dim3(64 * NW), smem, st, p);
   return LDM_OK;
 }
 
@@ -964,8 +971,8 @@ using namespace ldm;
 extern "C" int ldm_mx4_linear(const void* x, const void* x_scale, const void* w, const void* w_scale, const float* bias, void* out,
                               int out_dtype, long long rows, int n, int k, void* stream) {
   LDM_REQUIRE(dtype_ok(out_dtype), "ldm_mx4_linear: bad dtype %d", out_dtype);
-  LDM_REQUIRE(rows >= 0 && n >= 1 && k >= 1 && k <= (1 << 22), "ldm_mx4_linear: bad sizes (rows=%lld n=%d k=%d)", rows, n, k);
-  LDM_REQUIRE(rows < (1LL << 40) && ((rows + 63) / 64) * ((n + 63) / 64) < (1LL << 31), "ldm_mx4_linear: %lld x %d outputs are too many", rows, n);
+  LDM_REQUIRE(rows >= 0 && n >= 1 && n <= (1 << 30) && k >= 1 && k <= (1 << 22), "ldm_mx4_linear: bad sizes (rows=%lld n=%d k=%d)", rows, n, k);
+  LDM_REQUIRE(rows < (1LL << 40) && mx_tiles_launchable(rows, n), "ldm_mx4_linear: %lld x %d outputs are too many", rows, n);
   if (rows == 0) return LDM_OK;
   LDM_REQUIRE(x && w && w_scale && out, "ldm_mx4_linear: null pointer");
   const bool mx = x_scale != nullptr;
@@ -982,7 +989,6 @@ extern "C" int ldm_mx4_linear(const void* x, const void* x_scale, const void* w,
   p.tiles_m = p.tiles_n = 0;
   p.vec_out = aligned16(out) && (n * es) % 16 == 0;
   LDM_REQUIRE(rows <= 64LL * 65535 || mx, "ldm_mx4_linear: %lld rows of bfloat16", rows);
-  LDM_REQUIRE(((rows + 127) / 128) * ((n + 127LL) / 128) < (1LL << 31), "ldm_mx4_linear: too large (rows=%lld n=%d)", rows, n);
   hipStream_t st = (hipStream_t)stream;
   const int rc = out_dtype == LDM_BF16 ? mx4_linear_out<bf16_t>(p, mx, st) : mx4_linear_out<float>(p, mx, st);
   if (rc) return rc;
@@ -992,9 +998,9 @@ extern "C" int ldm_mx4_linear(const void* x, const void* x_scale, const void* w,
 
 extern "C" int ldm_linear_bf16(const void* x, const void* w, const float* bias, void* out, int out_dtype, long long rows, int n, int k, void* stream) {
   LDM_REQUIRE(dtype_ok(out_dtype), "ldm_linear_bf16: bad dtype %d", out_dtype);
-  LDM_REQUIRE(rows >= 0 && n >= 1 && k >= 8 && k % 8 == 0 && k <= (1 << 21), "ldm_linear_bf16: bad sizes (rows=%lld n=%d k=%d; k a multiple of 8)",
-              rows, n, k);
-  LDM_REQUIRE(rows < (1LL << 40) && ((rows + 63) / 64) * ((n + 63) / 64) < (1LL << 31), "ldm_linear_bf16: %lld x %d outputs are too many", rows, n);
+  LDM_REQUIRE(rows >= 0 && n >= 1 && n <= (1 << 30) && k >= 8 && k % 8 == 0 && k <= (1 << 21),
+              "ldm_linear_bf16: bad sizes (rows=%lld n=%d k=%d; k a multiple of 8)", rows, n, k);
+  LDM_REQUIRE(rows < (1LL << 40) && mx_tiles_launchable(rows, n), "ldm_linear_bf16: %lld x %d outputs are too many", rows, n);
   if (rows == 0) return LDM_OK;
   LDM_REQUIRE(x && w && out && aligned16(x) && aligned16(w) && (reinterpret_cast<uintptr_t>(bias) & 3) == 0 &&
                   reinterpret_cast<uintptr_t>(out) % dtype_size(out_dtype) == 0,
@@ -1018,8 +1024,7 @@ static int mx_rows_for_product(const char* what, const void** x, const void* w, 
                   (reinterpret_cast<uintptr_t>(w_scale) & 3) == 0 && (reinterpret_cast<uintptr_t>(bias) & 3) == 0 &&
                   reinterpret_cast<uintptr_t>(out) % dtype_size(out_dtype) == 0,
               "%s: null or unaligned pointer", what);
-  LDM_REQUIRE(rows < (1LL << 40) && outer <= (1 << 30) && ((rows + 63) / 64) * ((outer + 63) / 64) < (1LL << 31), "%s: %lld x %lld outputs are too many",
-              what, rows, outer);
+  LDM_REQUIRE(rows < (1LL << 40) && outer <= (1 << 30) && mx_tiles_launchable(rows, outer), "%s: %lld x %lld outputs are too many", what, rows, outer);
   const bool pad = ld != cols || !aligned16(*x);
   const long long need = (outer + (pad ? rows : 0)) * ld * 2;
   LDM_REQUIRE(workspace != nullptr && aligned16(workspace) && workspace_bytes >= need, "%s: workspace of %lld bytes needed (got %lld)", what, need,
