@@ -474,7 +474,7 @@ int ldm_mx4_linear_dgrad(const void* dy, const void* w, const void* w_scale, voi
                          long long workspace_bytes, void* stream);
 
 /* dw (n, k) float32 (+)= dY^T X: weight gradient of a linear layer whose input was kept in LDM_MX8.  dy (rows, n) bfloat16, contiguous,
- * 16-byte aligned, n a multiple of 8; x8 / x8_scale (rows, k).  Sums are float32 in a fixed order (no atomics).  `workspace` of
+ * 16-byte aligned, n a multiple of 8 below 2^24; x8 / x8_scale (rows, k), k up to 2^24.  Sums are float32 in a fixed order (no atomics).  `workspace` of
  * ldm_linear_wgrad_mx8_workspace_bytes (may be 0: NULL is fine then), 16-byte aligned. */
 long long ldm_linear_wgrad_mx8_workspace_bytes(long long rows, int n, int k);
 int ldm_linear_wgrad_mx8(const void* x8, const void* x8_scale, const void* dy, float* dw, long long rows, int n, int k, int accumulate,

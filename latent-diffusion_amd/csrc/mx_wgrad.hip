@@ -436,8 +436,9 @@ static int launch_wgrad_mx8(const WgradMx8Params& p, hipStream_t st) {
 
 using namespace ldm;
 
+// n, k: 64 rows of dY and of the checkpoint lie under descriptors of less than 2^31 bytes
 static bool wgrad_mx8_sizes_ok(long long rows, int n, int k) {
-  return rows >= 1 && rows <= 32LL * 0x7fffffff && n >= 1 && k >= 1 && n <= (1 << 24) && k <= (1 << 24) && (long long)n * k < (1LL << 38);
+  return rows >= 1 && rows <= 32LL * 0x7fffffff && n >= 1 && k >= 1 && n <= (1 << 24) - 8 && k <= (1 << 24) && (long long)n * k < (1LL << 38);
 }
 
 extern "C" long long ldm_linear_wgrad_mx8_workspace_bytes(long long rows, int n, int k) {

@@ -50,3 +50,16 @@ def test_products_of_too_many_outputs_are_refused():
     assert bad(lib.ldm_linear_bf16(p, p, 0, p, 1, 1 << 20, 1 << 19, 8, 0))
     assert bad(lib.ldm_mx4_linear_wide(p, p, p, 0, p, 1, 1 << 20, 1 << 19, 32, p, 1 << 60, 0))
     assert bad(lib.ldm_mx4_linear_dgrad(p, p, p, p, 1 << 20, 32, 1 << 19, p, 1 << 60, 0))
+
+
+def test_weight_gradient_of_rows_past_31_bits_is_refused():
+    """64 rows of dY are fetched under one 31-bit byte count."""
+    lib = _lib.load()
+    a = torch.zeros(4096, dtype=torch.uint8)
+    p = (a.data_ptr() + 15) // 16 * 16
+    widest = (1 << 24) - 8                                                                 # 64 rows: 2^31 - 1024 bytes
+    assert lib.ldm_linear_wgrad_mx8(p, p, p, p, 64, widest + 8, 32, 0, 0, 0, 0) == -1
+    assert b"bad sizes" in lib.ldm_last_error()
+    assert lib.ldm_linear_wgrad_mx8_workspace_bytes(1 << 20, widest + 8, 32) == 0
+    assert lib.ldm_linear_wgrad_mx8(p + 1, p, p, p, 64, widest, 32, 0, 0, 0, 0) == -1      # the sizes are fine, the pointer is not
+    assert b"unaligned" in lib.ldm_last_error()
