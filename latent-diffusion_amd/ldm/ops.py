@@ -1101,8 +1101,8 @@ def mx4_linear(x, w: MxTensor, bias: Optional[torch.Tensor] = None, out_dtype: O
     operands go to the matrix cores as they are -- or bfloat16 (*lead, k), contiguous, multiplied as it is with the weights widened
     (exactly) to bfloat16.  bias: float32 (n,).  out_dtype: bfloat16 (default) or float32."""
     _mx("mx4_linear: w", w, _lib.MX4)
-    if w.data.dim() != 2:
-        raise ValueError(f"mx4_linear: w must be (n, k), got {tuple(w.shape)}")
+    if w.data.dim() != 2 or w.data.shape[0] < 1:
+        raise ValueError(f"mx4_linear: w must be (n, k) with at least one row, got {tuple(w.shape)}")
     n, k = w.data.shape[0], w.cols
     mx = isinstance(x, MxTensor)
     if mx:
@@ -1142,8 +1142,8 @@ def mx4_linear_dgrad(dy: torch.Tensor, w: MxTensor) -> torch.Tensor:
     """Input gradient of mx4_linear(x, w): dy W, (*lead, n) -> (*lead, k), bfloat16, float32 sums.  The weights themselves have no
     gradient: they are frozen (what is trained around them -- biases, norms, added low-rank layers -- has its own operators)."""
     _mx("mx4_linear_dgrad: w", w, _lib.MX4)
-    if w.data.dim() != 2:
-        raise ValueError(f"mx4_linear_dgrad: w must be (n, k), got {tuple(w.shape)}")
+    if w.data.dim() != 2 or w.data.shape[0] < 1:
+        raise ValueError(f"mx4_linear_dgrad: w must be (n, k) with at least one row, got {tuple(w.shape)}")
     _gpu(dy)
     n, k = w.data.shape[0], w.cols
     if dy.dtype != torch.bfloat16:
