@@ -1228,10 +1228,16 @@ def linear_wgrad_mx8(x8: MxTensor, dy: torch.Tensor, *, out: Optional[torch.Tens
         full = torch.empty((npad, k), dtype=torch.float32, device=dy.device)
         _wgrad_mx8(x8, _pad_cols(dy.view(rows, n), npad), full, rows, npad, k, 0)
         full = full[:n]
-        return full if out is None else out.add_(full) if accumulate else out.copy_(full)
+        if out is None:
+            return full
+        # as storage, which is how the kernel writes into the ones of other widths: out may require a gradient itself
+        out.detach().add_(full) if accumulate else out.detach().copy_(full)
+        return out
     if out is None:
         out = torch.empty((n, k), dtype=torch.float32, device=dy.device)
     if rows == 0:
-        return out if accumulate else out.zero_()
+        if not accumulate:
+            out.detach().zero_()
+        return out
     _wgrad_mx8(x8, dy, out, rows, n, k, 1 if accumulate else 0)
     return out

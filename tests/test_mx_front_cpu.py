@@ -23,3 +23,18 @@ def test_weights_without_rows_are_refused():
             with pytest.raises(ValueError, match="at least one row"):
                 call()
         assert emu_lib().emu_launch_count() == before
+
+
+@pytest.mark.parametrize("rows,n", [(5, 16), (5, 13), (0, 16)])
+def test_weight_gradient_into_a_tensor_that_requires_grad(rows, n):
+    """Every width writes into ``out`` the way conv_wgrad does: as storage, whatever autograd knows of it."""
+    x, dy = seeded((rows, 40), 1).to(bf), seeded((rows, n), 2).to(bf)
+    with emulated() as ops:
+        x8 = ops.mx8_quantize(x)
+        want = ops.linear_wgrad_mx8(x8, dy)
+        out = torch.ones(n, 40, requires_grad=True)
+        assert ops.linear_wgrad_mx8(x8, dy, out=out, accumulate=False).data_ptr() == out.data_ptr()
+        assert torch.equal(out.detach(), want)
+        ops.linear_wgrad_mx8(x8, dy, out=out)
+        assert torch.equal(out.detach(), want + want)
+        assert out.is_leaf and out.requires_grad
