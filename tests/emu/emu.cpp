@@ -82,7 +82,7 @@ const std::function<void()>* g_body = nullptr;
 unsigned char* g_smem_map = nullptr;
 size_t g_smem_map_bytes = 0;
 unsigned char* g_smem = nullptr;
-int g_dma_lazy = 1;
+int g_dma_lazy = 1, g_dry_run = 0;
 long long g_launches = 0, g_waveops = 0;
 uint64_t g_clock = 0;
 
@@ -476,6 +476,7 @@ void wait_vmcnt(int n) {
 }
 
 void launch(dim3 grid, dim3 block, size_t dyn_smem_bytes, const std::function<void()>& body) {
+  if (g_dry_run) return;
   const int nthreads = (int)(block.x * block.y * block.z);
   if (nthreads < 1 || nthreads > MAX_THREADS) die("bad workgroup size");
   if (dyn_smem_bytes > 160 * 1024) die("more than 160 KiB of dynamic LDS");
@@ -512,6 +513,7 @@ void launch(dim3 grid, dim3 block, size_t dyn_smem_bytes, const std::function<vo
 extern "C" {
 
 void emu_set_dma_mode(int lazy) { emu::g_dma_lazy = lazy ? 1 : 0; }
+void emu_set_dry_run(int dry) { emu::g_dry_run = dry; }
 
 struct GuardHeader { void* map; size_t map_bytes; };
 static std::map<void*, GuardHeader> g_guarded;

@@ -65,6 +65,8 @@ uint64_t clock_ticks();
 extern "C" {
 // 0: eager (a DMA lands when it is issued), 1: lazy (when a counted wait retires it).  Default 1.
 void emu_set_dma_mode(int lazy);
+// != 0: launches are noted in the histogram and not executed (which kernel a call selects, at any size).  Default 0.
+void emu_set_dry_run(int dry);
 // [ptr, ptr + bytes) with PROT_NONE pages on both sides; ptr + bytes is the end of the last mapped page (bytes is rounded up
 // to 16 first), so the first byte past the end faults.  emu_free_guarded releases it.
 void* emu_alloc_guarded(size_t bytes);
