@@ -937,8 +937,9 @@ static float tile_rounds(const Mx4Params& p, int bm, int bn) {
 template <typename OUT>
 static int mx4_linear_out(Mx4Params& p, bool mx, hipStream_t st) {
   if (!mx) return p.k % 8 == 0 && aligned16(p.x) ? rows_by_size<false, true, OUT>(p, st) : rows_by_size<false, false, OUT>(p, st);
-  // few rows, or few enough outputs that each CU has at most one workgroup of the few-row kernel: 128 x 1280 (k = 1280) 3.5 us against 5.9 in
-  // tiles; with more, its re-reading of the operands loses: 128 x 10240 (k = 1280) 10.4 / 8.7
+  // few rows, or few enough outputs that each CU has at most one workgroup of the few-row kernel (k = 128 .. 8192: 128 x 1280 3.4 .. 8.8 us
+  // against 6.2 .. 12.1 in tiles, 1024 x 256 3.4 .. 10.6 / 6.2 .. 12.4); with two a CU its re-reading of the operands loses for longer sums
+  // (128 x 4096: k = 320 5.0 / 6.4, k = 1280 6.5 / 6.3, k = 8192 18.4 / 12.5)
   if (p.rows <= 64 || ((p.rows + 63) / 64) * ((p.n + 15) / 16) <= 256) return rows_by_size<true, true, OUT>(p, st);
   // rounds of one workgroup a CU x the time of 256 columns of the tile (us: 64 x 64 with its columns split 0.55, 128 x 128 1, 256 x 256
   // 2.3).  8192^3: 715, 464 and 341 us; 2048^3: 21.5, 11.5, 12.3; 154 x 2560 (k = 2560): 7.3, 10.4, 12.0

@@ -1072,11 +1072,15 @@ def mx_dequantize(q: MxTensor, dtype: torch.dtype) -> torch.Tensor:
     return out
 
 
-def _mx4_widen_once(rows: int, n: int) -> bool:
+def _mx4_widen_once(rows: int, n: int, k: int) -> bool:
     """bf16 activations: whether the weights are widened once to memory, or in registers, by workgroups of 64 rows and 16 outputs.
-    In registers up to 256 rows (1280 on 10240 outputs: 24.9 us against 29.2; 384 rows 36.9 / 29.0), and while such workgroups are few
-    (512 rows of 1280 on 320 outputs 5.9 / 12.3, on 1280 outputs 12.8 / 14.2; 2560 on 2560 28.7 / 28.6)."""
-    return rows > 256 and ((rows + 63) // 64) * ((n + 15) // 16) > 960
+    In registers up to 256 rows (k = 128 .. 8192, us: 1280 outputs 5.7 .. 28 against 8.9 .. 35, 8192 outputs 11 .. 66 / 9.8 .. 77); beyond,
+    while such workgroups are few (k = 1280: 512 rows on 1280 outputs 13.6 / 14.7, on 1920 17.0 / 16.1, on 2560 21.2 / 19.2) and so is what
+    they read of x again for every 16 outputs but the first (512 rows on 1280: k = 2560 18.9 / 20.4, k = 8192 40 / 35; 4096 rows on 160: k = 320
+    9.8 / 9.4, k = 1280 18.1 / 13.1, k = 8192 76 / 31; 8000 rows on 32: k = 1280 9.6 / 13.0, k = 5120 25.7 / 24.9; 30000 rows on 16: k = 5120
+    57 / 63).  The product behind the widening takes 2^21 columns, the other 2^22."""
+    down, across = (rows + 63) // 64, (n + 15) // 16
+    return rows > 256 and k <= 1 << 21 and (down * across > 960 or down * (across - 1) * rows * k > 1_300_000_000)
 
 
 def _pad_cols(t: torch.Tensor, cols: int) -> torch.Tensor:
@@ -1125,7 +1129,7 @@ def mx4_linear(x, w: MxTensor, bias: Optional[torch.Tensor] = None, out_dtype: O
     _same_device("mx4_linear", xt, w.data, bias)
     lead = xt.shape[:-1]
     rows = xt.numel() // xt.shape[-1]
-    if not mx and _mx4_widen_once(rows, n):
+    if not mx and _mx4_widen_once(rows, n, k):
         out = torch.empty((*lead, n), dtype=odt, device=x.device)
         ws, need = _widening_workspace(x, rows, k, n)
         _call(x, "ldm_mx4_linear_wide", x.data_ptr(), w.data.data_ptr(), w.scale.data_ptr(), _ptr(bias), out.data_ptr(), code, rows, n, k,

@@ -67,7 +67,9 @@ BF16 = [
     (300, 130, 1300, "mx4_rows_kernel<false, 4, 1, 4, 2, false"),
     (40, 4100, 136, "mx4_rows_kernel<false, 4, 2, 4, 2, true"),
     (40, 4100, 137, "mx4_rows_kernel<false, 4, 2, 4, 2, false"),
+    (4000, 16, 64, "mx4_rows_kernel<false, 4, 1, 4, 2, true"),
     # widened once
+    (4000, 160, 1288, "mx_gemm_kernel<64, 64, 1, 1, 4, 2, false"),       # few workgroups, but a large x
     (300, 3200, 1100, "mx_gemm_kernel<64, 64, 1, 1, 4, 2, false"),
     (300, 3201, 2101, "mx_gemm_kernel<64, 64, 1, 1, 4, 2, false"),
     (66000, 16, 9, "mx_gemm_kernel<64, 64, 1, 1, 4, 2, false"),          # more rows to pad than a grid's second dimension has
