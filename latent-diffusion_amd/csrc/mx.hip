@@ -7,8 +7,9 @@
 //         bit), two to a byte, the lower column in the lower half: x -> nearest(x / 2^e), ties to the even code, at most 6
 //   mx8   e = max(floor(log2 a), -127), elements q / 64 with q = -127 .. 127: q = nearest_even(64 x / 2^e), at most 127
 // A block with an infinity or a NaN gets the byte 255 and stands for NaN throughout.  Scaling by a power of two is exact, so the
-// ONE rounding of an element is the format's own: at most half a step.  mx4: 2^-2 of the value for a / 2^e <= 6 (a quarter of it
-// for the values between 6 and 8, which are held to 6); mx8: a / 128, or a / 64 for the values between 127.5 / 64 and 2.
+// ONE rounding of an element is the format's own, by the block's scale and not by the element: small elements of a block may vanish.
+// mx4: at most 2^e / 4 below 2 2^e, 2^e / 2 below 4 2^e and 2^e up to 6 2^e, above which values (a may reach 8 2^e) are held to 6 2^e, up to
+// 2 2^e off; mx8: at most 2^e / 128, or 2^e / 64 for magnitudes past 127.5 / 64 2^e (a may reach 2 2^e), which are held to 127 / 64 2^e.
 // Storage: elements row-major without gaps between blocks (16 / 32 bytes a block), scale bytes row-major with rows filled up
 // with zeros to whole 32-bit words (mx_scale_stride), so that a matrix kernel can fetch four blocks' scales at once.
 //

@@ -6,9 +6,9 @@
 // and its scale byte; products and sums are float32 inside the instruction, so nothing is rounded before the output.  The weights
 // are the instruction's first operand: a lane then holds four consecutive n of one m.
 //   mx4_gemm_kernel   large outputs.  8192^3: 310-340 us, 3.2-3.5 PFLOP/s (a loop of this instruction alone on random operands, without
-//                     any loads: 6.4); 32768 x 2560, k = 320: 50 us, 168 MB of output at 3.4 TB/s.
+//                     any loads: 6.4); 32768 x 2560, k = 320: 51 us, 168 MB of output at 3.3 TB/s.
 //   mx_gemm_kernel    small and medium outputs, and plain bf16 operands (the product behind the widening of the weights): 8192 x 640, k =
-//                     5120 in bf16: 66 us, 810 TFLOP/s; 154 x 768, k = 1312: 6.9 us.
+//                     5120 in bf16: 60 us, 890 TFLOP/s; 154 x 768, k = 1312: 7.5 us.
 //   mx4_rows_kernel   few rows of x, where the weights' bytes are what counts: 16 x 10240, k = 8192: 13 us, 3.3 TB/s.
 #include "common.h"
 
@@ -389,8 +389,9 @@ mx4_gemm_kernel(const Mx4Params p) {
 // (zeros), rows past the end likewise, and steps past the end too: their number is rounded up to an even one.
 //
 // S slots of LDS.  The registers of a whole step -- four rounds of matrix instructions -- are read while the step before multiplies, reads and
-// DMA spread between the instructions, one barrier a step.  What bounds the loop is LDS: a wave's tile of 64 x 64 reads as many bytes as its
-// instructions take time, 64 x 128 or 64 x 160 fewer.
+// DMA spread between the instructions, one barrier a step.  What bounds the loop is LDS: a wave's tile of 64 x 64 reads 0.031 rows of
+// operands a product, which takes as long as its instructions; the 64 x 160 of the 256 x 160 tile reads 0.022, but the 32 x 160 of the
+// 128 x 160 tile 0.0375.
 //   KW == 1: WM x WN waves share the tile.
 //   KW > 1:  few tiles, where a launch is as long as one workgroup's chain of steps: the KW waves of a workgroup each take a contiguous part
 //            of the columns of the whole tile, with a ring of their own and no barrier, and add up through LDS in a fixed order.
