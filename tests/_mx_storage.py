@@ -1,6 +1,7 @@
 """Bodies of tests/test_mx_storage_cpu.py and tests/test_mx_storage_gpu.py: what a row's storage holds behind its last column."""
 import torch
 
+from _mx_paths import exact4
 from conftest import seeded
 
 bf = torch.bfloat16
@@ -20,7 +21,7 @@ def stored(ops, x, cols, dev):
     return clean, dirty
 
 
-def check_product(ops, rows, n, k, act, dev, one_by_one=True):
+def check_product(ops, rows, n, k, act, dev):
     """A product of rows with anything behind their last column has the bits of the one with zeros there."""
     wide = -(-k // 128) * 128
     w, w_dirty = stored(ops, seeded((n, wide), 5), k, dev)
@@ -30,8 +31,16 @@ def check_product(ops, rows, n, k, act, dev, one_by_one=True):
         x = x_dirty = dev(seeded((rows, k), 6).to(bf))
     want = ops.mx4_linear(x, w, out_dtype=torch.float32)
     assert torch.isfinite(want).all()
-    for a, b in ((x_dirty, w_dirty), (x_dirty, w), (x, w_dirty))[: 3 if one_by_one else 1]:
+    for a, b in ((x_dirty, w_dirty), (x_dirty, w), (x, w_dirty)):
         assert torch.equal(ops.mx4_linear(a, b, out_dtype=torch.float32), want)
+
+
+def check_exact_product(ops, rows, n, k, dev):
+    """One product of 4-bit rows with anything behind their last column, against sums that are exact (_mx_paths.exact4)."""
+    wide = -(-k // 128) * 128
+    x, w = exact4(rows, wide, 1), exact4(n, wide, 2)
+    got = ops.mx4_linear(stored(ops, x, k, dev)[1], stored(ops, w, k, dev)[1], out_dtype=torch.float32)
+    assert torch.equal(got.cpu(), x[:, :k] @ w[:, :k].t())
 
 
 def check_other_readers(ops, dev):

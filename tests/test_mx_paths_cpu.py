@@ -93,15 +93,15 @@ def test_every_kernel_of_the_library_has_a_case(launched, tmp_path):
 def test_long_rows_run_in_registers(launched):
     """The product of widened weights takes 2^21 columns, the one in registers 2^22."""
     with emulated() as ops:
-        for k in ((1 << 21) + 1, 1 << 22):
-            assert launched(_linear, ops, "bf16", 300, 16, k, bf) == {f"mx4_rows_kernel<false, 4, 1, 4, 2, {'false' if k % 8 else 'true'}, unsigned short>"}
-        assert launched(_linear, ops, "bf16", 300, 4096, 1 << 22, bf) == {"mx4_rows_kernel<false, 4, 1, 4, 2, true, unsigned short>"}
-        assert "mx_dequantize_kernel<unsigned short, 4>" in launched(_linear, ops, "bf16", 300, 4096, 1 << 21, bf)
+        k = (1 << 21) + 8
+        assert launched(_linear, ops, "bf16", 257, 1, k, bf) == {"mx4_rows_kernel<false, 4, 1, 4, 2, true, unsigned short>"}
+        for rows, n in ((257, 1), (300, 4096), (100000, 4096)):
+            assert not ops._mx4_widen_once(rows, n, k) and ops._mx4_widen_once(rows, max(n, 4096), k - 8)
 
 
 def _both_dma(cases):
     """(rows, n, k, DMA completion model): both models where that takes seconds."""
-    return [(*c[:3], dma) for c in cases for dma in ("lazy", "eager") if dma == "lazy" or c[0] * c[1] * c[2] < 1.2e9]
+    return [(*c[:3], dma) for c in cases for dma in ("lazy", "eager") if dma == "lazy" or c[0] * c[1] * c[2] < 5e8]
 
 
 @pytest.mark.parametrize("rows,n,k,dma", _both_dma(paths.MX4))

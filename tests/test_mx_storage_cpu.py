@@ -18,18 +18,25 @@ def test_product_few_rows(rows, n, k, act):
         storage.check_product(ops, rows, n, k, act, g.like)
 
 
-# 64 x 64 with its columns split, 128 x 128, 256 x 128
 @pytest.mark.parametrize("dma", ["lazy", "eager"])
-@pytest.mark.parametrize("rows,n,k", [(290, 900, 77), (290, 900, 160), (290, 901, 333), (1030, 1410, 45), (1030, 1410, 297), (2050, 4104, 70), (2050, 4104, 96)])
-def test_product_tiles(rows, n, k, dma):
+@pytest.mark.parametrize("rows,n,k", [(290, 900, 77), (290, 900, 160), (290, 901, 333)])
+def test_product_tiles_with_columns_split(rows, n, k, dma):
     with Guarded() as g, emulated(dma, guard=True) as ops:
         storage.check_product(ops, rows, n, k, "mx4", g.like)
+
+
+# 128 x 128, 256 x 128
+@pytest.mark.parametrize("rows,n,k,dma", [(1030, 1410, 45, "lazy"), (1030, 1410, 297, "eager"), (1030, 1410, 352, "lazy"), (2050, 4104, 70, "lazy"),
+                                          (2050, 4104, 96, "eager")])
+def test_product_tiles(rows, n, k, dma):
+    with Guarded() as g, emulated(dma, guard=True) as ops:
+        storage.check_exact_product(ops, rows, n, k, g.like)
 
 
 def test_product_largest_tile():
     """256 x 256, taken for sums of 2048 columns and more."""
     with Guarded() as g, emulated(guard=True) as ops:
-        storage.check_product(ops, 2050, 4104, 2057, "mx4", g.like, one_by_one=False)
+        storage.check_exact_product(ops, 2050, 4104, 2057, g.like)
 
 
 def test_other_readers():

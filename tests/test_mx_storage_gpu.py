@@ -19,5 +19,10 @@ def test_product(rows, n, k, act):
     storage.check_product(ops, rows, n, k, act, dev)
 
 
+@pytest.mark.parametrize("rows,n,k", [(3, 40, 45), (290, 901, 3333), (1030, 1410, 297), (2050, 4104, 70), (2050, 4104, 2057)])
+def test_exact_product(rows, n, k):
+    storage.check_exact_product(ops, rows, n, k, dev)
+
+
 def test_other_readers():
     storage.check_other_readers(ops, dev)
