@@ -6,6 +6,7 @@ Activations are NHWC: a tensor of shape (B, H, W, C) or (B, L, C), contiguous.
 from __future__ import annotations
 
 import ctypes as C
+import operator
 from typing import Optional
 
 import torch
@@ -964,13 +965,14 @@ class MxTensor:
     __slots__ = ("data", "scale", "cols")
 
     def __init__(self, data: torch.Tensor, scale: torch.Tensor, cols: int):
+        cols = operator.index(cols)
         blocks = (cols + 31) // 32
         if cols < 1 or data.dim() < 1 or data.dtype not in (torch.uint8, torch.int8):
             raise TypeError(f"MxTensor: data must be uint8 (4-bit) or int8 (8-bit) rows of at least one column (got {data.dtype})")
         if scale.dtype != torch.uint8:
             raise TypeError(f"MxTensor: scale must be uint8 (got {scale.dtype})")
         width = blocks * (16 if data.dtype == torch.uint8 else 32)
-        if data.shape[-1] != width or scale.shape[-1] != (blocks + 3) // 4 * 4 or data.shape[:-1] != scale.shape[:-1]:
+        if scale.dim() < 1 or data.shape[-1] != width or scale.shape[-1] != (blocks + 3) // 4 * 4 or data.shape[:-1] != scale.shape[:-1]:
             raise ValueError(f"MxTensor: {cols} columns need rows of {width} elements' bytes and {(blocks + 3) // 4 * 4} scales "
                              f"(got {tuple(data.shape)} and {tuple(scale.shape)})")
         if data.device != scale.device:

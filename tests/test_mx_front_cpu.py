@@ -38,3 +38,13 @@ def test_weight_gradient_into_a_tensor_that_requires_grad(rows, n):
         ops.linear_wgrad_mx8(x8, dy, out=out)
         assert torch.equal(out.detach(), want + want)
         assert out.is_leaf and out.requires_grad
+
+
+def test_mx_tensor_refuses_a_scalar_scale_and_a_fractional_width():
+    with emulated() as ops:
+        data, scale = torch.zeros(16, dtype=torch.uint8), torch.zeros(4, dtype=torch.uint8)
+        assert ops.MxTensor(data, scale, 32).shape == (32,)
+        with pytest.raises(ValueError):
+            ops.MxTensor(data, scale[0], 32)
+        with pytest.raises(TypeError):
+            ops.MxTensor(data, scale, 32.0)
